@@ -34,6 +34,7 @@ extern "C" {
 
 #define Y5M_F32 0
 #define Y5M_BF16 1
+#define Y5M_F16 2              /* the channels-last operators below (y5m_gn_act*, y5m_act8_*) only */
 
 /* activation flags for epilogues */
 #define Y5M_ACT_NONE 0
@@ -437,6 +438,19 @@ size_t y5m_adam_workspace_bytes(void);
 int y5m_grad_norm(const float* g, int64_t n, float* norm_out, void* ws, size_t ws_bytes, void* stream);
 int y5m_adam_step(float* p, const float* g, float* m, float* v, int64_t n, const float* gnorm, float max_norm,
                   double lr, double beta1, double beta2, double eps, double weight_decay, const int32_t* d_step,
+                  void* stream);
+
+/* ---- activations kept in 8 bits ----------------------------------------------------------------------------------------------
+ * A row of C channels is held as blocks of 32 channels: codes q [row][ldq] (1 byte each, ldq % 8 == 0, the tail of a row's last
+ * 8-byte piece zero) and one byte e + 127 per block, scale [row][ceil(C / 32)]; a code stands for (e4m3 or int8 value) * 2^e, with
+ * e the smallest exponent that holds the block's largest |x| (>= -117), codes rounded to nearest even. A block with a value that is
+ * not finite has scale byte 255 and reads back as NaN. dtype: Y5M_F32 / Y5M_BF16 / Y5M_F16. Rows: element strides, channels dense. */
+#define Y5M_KEEP_NONE 0
+#define Y5M_KEEP_E4M3 1
+#define Y5M_KEEP_INT8 2
+int y5m_act8_store(const void* x, int64_t x_batch_stride, int64_t x_row_stride, int64_t N, int64_t S, int C, void* q, int ldq,
+                   void* scale, int fmt, int dtype, void* stream);
+int y5m_act8_load(const void* q, int ldq, const void* scale, int64_t M, int C, void* x, int64_t x_row_stride, int fmt, int dtype,
                   void* stream);
 
 #ifdef __cplusplus

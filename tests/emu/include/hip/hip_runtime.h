@@ -286,6 +286,33 @@ static inline float __builtin_amdgcn_rsqf(float x) { return 1.0f / sqrtf(x); }
 static inline float __builtin_amdgcn_exp2f(float x) { return exp2f(x); }
 static inline const void* __builtin_amdgcn_kernarg_segment_ptr() { return emu::g.kernarg; }
 
+// OCP fp8 e4m3 (bias 7, largest 448, subnormals in steps of 2^-9, 0x7f / 0xff NaN): round to nearest even; beyond 448 + half a step NaN
+static inline unsigned emu_f32_to_e4m3(float f) {
+    const unsigned s = __builtin_bit_cast(unsigned, f) >> 31 << 7;
+    const float a = __builtin_fabsf(f);
+    if (!(a <= 464.0f)) return s | 0x7fu;
+    if (a < 0.015625f) return s | (unsigned)__builtin_rintf(a * 512.0f);
+    int ex = (int)(__builtin_bit_cast(unsigned, a) >> 23) - 127;
+    unsigned m = (unsigned)__builtin_rintf(__builtin_ldexpf(a, 3 - ex));       // 8 .. 16
+    if (m == 16) { m = 8; ++ex; }
+    const unsigned code = (unsigned)(ex + 7) << 3 | (m - 8);
+    return s | (code > 0x7eu ? 0x7fu : code);
+}
+static inline float emu_e4m3_to_f32(unsigned b) {
+    const unsigned e = (b >> 3) & 15, m = b & 7;
+    const float a = e == 15 && m == 7 ? __builtin_nanf("") : e ? __builtin_ldexpf((float)(8 + m), (int)e - 10) : (float)m / 512.0f;
+    return b & 0x80 ? -a : a;
+}
+typedef float emu_f32x2 __attribute__((ext_vector_type(2)));
+static inline int __builtin_amdgcn_cvt_pk_fp8_f32(float a, float b, int old, bool hi) {
+    const unsigned p = emu_f32_to_e4m3(a) | emu_f32_to_e4m3(b) << 8;
+    return (int)(hi ? ((unsigned)old & 0xffffu) | p << 16 : ((unsigned)old & 0xffff0000u) | p);
+}
+static inline emu_f32x2 __builtin_amdgcn_cvt_pk_f32_fp8(int v, bool hi) {
+    const unsigned p = (unsigned)v >> (hi ? 16 : 0);
+    return emu_f32x2{emu_e4m3_to_f32(p & 0xff), emu_e4m3_to_f32(p >> 8 & 0xff)};
+}
+
 // DPP: the four controls the kernels use, row_mask = bank_mask = 0xF, bound_ctrl: quad_perm [1,0,3,2] (0xB1),
 // quad_perm [2,3,0,1] (0x4E), row_half_mirror (0x141), row_mirror (0x140)
 static inline int __builtin_amdgcn_update_dpp(int old, int v, int ctrl, int row_mask, int bank_mask, bool bound_ctrl) {
