@@ -451,7 +451,26 @@ int y5m_adam_step(float* p, const float* g, float* m, float* v, int64_t n, const
 int y5m_act8_store(const void* x, int64_t x_batch_stride, int64_t x_row_stride, int64_t N, int64_t S, int C, void* q, int ldq,
                    void* scale, int fmt, int dtype, void* stream);
 int y5m_act8_load(const void* q, int ldq, const void* scale, int64_t M, int C, void* x, int64_t x_row_stride, int fmt, int dtype,
-                  void* stream);
+                  void* stream);/* weight gradient of a pointwise convolution from its input in 8 bits: dw[n][c] = sum over the N * S rows of dy[row][n] * value[row][c]
+ * (f32, [Cout][C], OVERWRITTEN); db[n] = sum of dy[row][n] (NULL: not wanted). dtype: dy's. No atomics, one result per input. */
+size_t y5m_act8_wgrad_workspace_bytes(int64_t M, int Cout, int C);
+int y5m_act8_wgrad(const void* dy, int64_t dy_batch_stride, int64_t dy_row_stride, int64_t N, int64_t S, int Cout, const void* q, int ldq,
+                   const void* scale, int C, int fmt, float* dw, float* db, void* ws, size_t ws_bytes, int dtype, void* stream);
+
+/* ---- group normalisation + activation over channels-last rows -------------------------------------------------------------------
+ * N samples of S rows of C channels in G groups; strides in elements, channels dense, any strides for inputs (views of wider
+ * buffers); gamma / beta may be NULL (1, 0). mean / rstd [N][G] f32 are outputs of the forward and inputs of the backward.
+ * fmt != Y5M_KEEP_NONE: the forward also writes the 8-bit form of x (q, scale; row = n * S + s) and the backward reads it instead of x.
+ * z may be x itself (equal strides). The backward OVERWRITES dgamma / dbeta (NULL: not wanted); no atomics, one result per input. */
+size_t y5m_gn_act_workspace_bytes(int64_t N, int64_t S, int C, int G);
+int y5m_gn_act(const void* x, int64_t x_batch_stride, int64_t x_row_stride, const float* gamma, const float* beta, int64_t N, int64_t S,
+               int C, int G, float eps, int act, void* z, int64_t z_batch_stride, int64_t z_row_stride, float* mean, float* rstd, void* q,
+               int ldq, void* scale, int fmt, void* ws, size_t ws_bytes, int dtype, void* stream);
+size_t y5m_gn_act_bwd_workspace_bytes(int64_t N, int64_t S, int C, int G);
+int y5m_gn_act_bwd(const void* dz, int64_t dz_batch_stride, int64_t dz_row_stride, const void* x, int64_t x_batch_stride,
+                   int64_t x_row_stride, const void* q, int ldq, const void* scale, int fmt, const float* gamma, const float* beta,
+                   const float* mean, const float* rstd, int64_t N, int64_t S, int C, int G, int act, void* dx, int64_t dx_batch_stride,
+                   int64_t dx_row_stride, float* dgamma, float* dbeta, void* ws, size_t ws_bytes, int dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -154,6 +154,7 @@ static void run_block(Dim3 bid, Dim3 grid, Dim3 block, const void* kernarg) {
         Wave& W = P.waves[w];
         W.n = (w == nwaves - 1) ? nthreads - 64 * w : 64;
         W.parity = 0;
+        W.present[0] = W.present[1] = 0;
         for (int i = 0; i < W.n; ++i) W.lanes[i] = &P.lanes[64 * w + i];
     }
     // Y5M_EMU_WAVE_ORDER: the order in which the scheduler visits the waves of a workgroup -- 0 ascending (default), 1
@@ -208,6 +209,7 @@ static void run_block(Dim3 bid, Dim3 grid, Dim3 block, const void* kernarg) {
                     abort();
                 }
                 W.parity ^= 1;
+                W.present[W.parity] = 0;
                 for (int i = 0; i < W.n; ++i)
                     if (W.lanes[i]->state == AT_COLLECTIVE) W.lanes[i]->state = RUNNABLE;
                 progress = true;

@@ -64,6 +64,7 @@ struct Lane {
 struct Wave {
     Lane* lanes[64];
     int n, parity;
+    unsigned long long present[2];      // lanes that deposited for the collective of this parity (a lane that ends right behind one was there)
     alignas(16) unsigned char slot[2][64][SLOT_BYTES];
 };
 
@@ -84,10 +85,11 @@ struct Coll {
     int p, lane;
     template <typename T> T& mine() { return *reinterpret_cast<T*>(w->slot[p][lane]); }
     template <typename T> const T& of(int l) const { return *reinterpret_cast<const T*>(w->slot[p][l]); }
-    bool live(int l) const { return l < w->n && w->lanes[l]->state != DONE; }
+    bool live(int l) const { return l < w->n && (w->present[p] >> l & 1); }
 };
 inline Coll coll_begin() {
     Lane* l = g.cur;
+    l->wave->present[l->wave->parity] |= 1ull << l->lane;
     return Coll{l->wave, l->wave->parity, l->lane};
 }
 inline void coll_sync(int op) {

@@ -13,7 +13,10 @@ from .model import YOLOV5m  # noqa: F401
 from .ultralytics_loss import ComputeLoss  # noqa: F401
 from .loss import YOLO_LOSS  # noqa: F401
 from .utils.plot_utils import cells_to_bboxes, make_grids  # noqa: F401
+from .act8 import Act8, act8_load, act8_store, act8_wgrad  # noqa: F401
+from .group_norm import GroupNormAct, group_norm_act, group_norm_act_backward  # noqa: F401
 from .utils.bboxes_utils import non_max_suppression, intersection_over_union, iou_width_height  # noqa: F401
 
 __all__ = ["YOLOV5m", "ComputeLoss", "YOLO_LOSS", "cells_to_bboxes", "make_grids", "non_max_suppression",
-           "intersection_over_union", "iou_width_height", "config"]
+           "intersection_over_union", "iou_width_height", "config", "Act8", "act8_store", "act8_load", "act8_wgrad",
+           "GroupNormAct", "group_norm_act", "group_norm_act_backward"]

@@ -24,12 +24,21 @@ from .arch import cbl_list
 
 
 class CBL(nn.Module):
-    """reference model.py:12-28 (parameter container; BN eps=1e-3, momentum=0.03)"""
+    """reference model.py:12-28 (parameter container; BN eps=1e-3, momentum=0.03)
 
-    def __init__(self, in_channels, out_channels, kernel_size, stride, padding):
+    norm_groups: GroupNorm over that many groups in BatchNorm's place (statistics of one image: small batches), for blocks built from
+    these modules; the whole-model engine runs the BatchNorm network. keep (with norm_groups): what a training forward leaves for its
+    backward -- "x" (the convolution's input and output whole) or "e4m3" / "int8" (both in 8 bits, act8.py)."""
+
+    def __init__(self, in_channels, out_channels, kernel_size, stride, padding, norm_groups=None, keep="x"):
         super().__init__()
         conv = nn.Conv2d(in_channels, out_channels, kernel_size, stride, padding, bias=False)
-        bn = nn.BatchNorm2d(out_channels, eps=1e-3, momentum=0.03)
+        self.norm_groups = norm_groups
+        if norm_groups is None:
+            bn = nn.BatchNorm2d(out_channels, eps=1e-3, momentum=0.03)
+        else:
+            from .group_norm import GroupNormAct
+            bn = GroupNormAct(norm_groups, out_channels, eps=1e-3, act="silu", keep=keep)
         self.cbl = nn.Sequential(conv, bn, nn.SiLU(inplace=True))
 
     compute_dtype = "f32"        # sub-module execution: "f32" (parity) or "bf16"; per instance or on the class
@@ -39,7 +48,64 @@ class CBL(nn.Module):
         eval mode the running statistics; differentiable wrt the input and the parameters (one autograd node, `_CBLFn`)"""
         _lib.require_cuda(x)
         conv, bn = self.cbl[0], self.cbl[1]
+        if self.norm_groups is not None:
+            return bn(_ConvKeptFn.apply(x.float(), conv.weight, self)).float()
         return _CBLFn.apply(x.float(), conv.weight, bn.weight, bn.bias, self)
+
+
+class _ConvKeptFn(torch.autograd.Function):
+    """the convolution of a CBL with GroupNorm: its output stays channels last for the norm, its input is kept for the weight gradient
+    whole or in 8 bits (act8_store). A 1x1 stride-1 convolution takes the weight gradient from the 8-bit form (act8_wgrad), any other
+    from the values read back (act8_load)"""
+
+    @staticmethod
+    def forward(ctx, x, w, mod):
+        from . import ops
+        from .act8 import act8_store
+        conv, keep, dtype = mod.cbl[0], mod.cbl[1].keep, mod.compute_dtype
+        k, s, p = conv.kernel_size[0], conv.stride[0], conv.padding[0]
+        ch = 8 if dtype == "bf16" else 4
+        cin = x.shape[1]
+        xd, wd = x.detach().float(), w.detach().float()
+        if cin % ch:                                          # zero channels up to a 16-byte piece
+            padc = ch - cin % ch
+            xd = torch.nn.functional.pad(xd, (0, 0, 0, 0, 0, padc))
+            wd = torch.nn.functional.pad(wd, (0, 0, 0, 0, 0, padc))
+        tdt = torch.bfloat16 if dtype == "bf16" else torch.float32
+        y = ops.conv_forward(xd, wd, s, p, dtype).to(tdt).contiguous(memory_format=torch.channels_last)
+        ctx.geom = (k, s, p, dtype, cin, tuple(x.shape[2:]))
+        ctx.act8 = None
+        kept = [None, None]
+        if ctx.needs_input_grad[1]:                           # (the input is read by the weight gradient only)
+            if keep == "x":
+                kept = [xd, None]
+            else:
+                a = act8_store(xd.to(tdt).contiguous(memory_format=torch.channels_last), keep)
+                ctx.act8 = (a.shape, a.dtype, a.fmt)
+                kept = [a.q, a.scale]
+        ctx.save_for_backward(wd, *kept)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        from . import ops
+        from .act8 import Act8, act8_load, act8_wgrad
+        wd, xk, scale = ctx.saved_tensors
+        k, s, p, dtype, cin, hw = ctx.geom
+        dx = dw = None
+        if ctx.needs_input_grad[0]:
+            dx = ops.conv_dgrad(dy.float(), wd, hw, s, p, dtype)[:, :cin]
+        if ctx.needs_input_grad[1]:
+            if ctx.act8 is None:
+                dw = ops.conv_wgrad(dy.float(), xk, k, s, p, dtype)
+            elif k == 1 and s == 1 and p == 0:
+                dw, _ = act8_wgrad(dy.contiguous(memory_format=torch.channels_last), Act8(xk, scale, *ctx.act8))
+                dw = dw[:, :, None, None]
+            else:
+                dw = ops.conv_wgrad(dy.float(), act8_load(Act8(xk, scale, *ctx.act8)).float(), k, s, p, dtype)
+            dw = dw[:, :cin]
+        return dx, dw, None
 
 
 class _CBLFn(torch.autograd.Function):
@@ -102,13 +168,13 @@ class _CBLFn(torch.autograd.Function):
 
 
 class Bottleneck(nn.Module):
-    """reference model.py:32-50"""
+    """reference model.py:32-50 (norm: CBL's norm_groups / keep)"""
 
-    def __init__(self, in_channels, out_channels, width_multiple=1):
+    def __init__(self, in_channels, out_channels, width_multiple=1, **norm):
         super().__init__()
         c_ = int(width_multiple * in_channels)
-        self.c1 = CBL(in_channels, c_, kernel_size=1, stride=1, padding=0)
-        self.c2 = CBL(c_, out_channels, kernel_size=3, stride=1, padding=1)
+        self.c1 = CBL(in_channels, c_, kernel_size=1, stride=1, padding=0, **norm)
+        self.c2 = CBL(c_, out_channels, kernel_size=3, stride=1, padding=1, **norm)
 
     def forward(self, x):
         """reference model.py:49-50"""
@@ -116,18 +182,18 @@ class Bottleneck(nn.Module):
 
 
 class C3(nn.Module):
-    """reference model.py:54-92"""
+    """reference model.py:54-92 (norm: CBL's norm_groups / keep)"""
 
-    def __init__(self, in_channels, out_channels, width_multiple=1, depth=1, backbone=True):
+    def __init__(self, in_channels, out_channels, width_multiple=1, depth=1, backbone=True, **norm):
         super().__init__()
         c_ = int(width_multiple * in_channels)
-        self.c1 = CBL(in_channels, c_, kernel_size=1, stride=1, padding=0)
-        self.c_skipped = CBL(in_channels, c_, kernel_size=1, stride=1, padding=0)
+        self.c1 = CBL(in_channels, c_, kernel_size=1, stride=1, padding=0, **norm)
+        self.c_skipped = CBL(in_channels, c_, kernel_size=1, stride=1, padding=0, **norm)
         if backbone:
-            self.seq = nn.Sequential(*[Bottleneck(c_, c_, width_multiple=1) for _ in range(depth)])
+            self.seq = nn.Sequential(*[Bottleneck(c_, c_, width_multiple=1, **norm) for _ in range(depth)])
         else:
-            self.seq = nn.Sequential(*[nn.Sequential(CBL(c_, c_, 1, 1, 0), CBL(c_, c_, 3, 1, 1)) for _ in range(depth)])
-        self.c_out = CBL(c_ * 2, out_channels, kernel_size=1, stride=1, padding=0)
+            self.seq = nn.Sequential(*[nn.Sequential(CBL(c_, c_, 1, 1, 0, **norm), CBL(c_, c_, 3, 1, 1, **norm)) for _ in range(depth)])
+        self.c_out = CBL(c_ * 2, out_channels, kernel_size=1, stride=1, padding=0, **norm)
 
     def forward(self, x):
         """reference model.py:90-92"""
