@@ -312,6 +312,21 @@ static inline emu_f32x2 __builtin_amdgcn_cvt_pk_f32_fp8(int v, bool hi) {
     const unsigned p = (unsigned)v >> (hi ? 16 : 0);
     return emu_f32x2{emu_e4m3_to_f32(p & 0xff), emu_e4m3_to_f32(p >> 8 & 0xff)};
 }
+typedef __bf16 emu_bf16x2 __attribute__((ext_vector_type(2)));
+// v_cvt_scalef32_pk_bf16_fp8: two e4m3 values times the power of two in the scale's exponent field (all ones: NaN), as bf16
+static inline emu_bf16x2 __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(unsigned v, float scale, bool hi) {
+    const emu_f32x2 f = __builtin_amdgcn_cvt_pk_f32_fp8((int)v, hi);
+    const unsigned e = __builtin_bit_cast(unsigned, scale) >> 23 & 255;
+    const float s = e == 255 ? __builtin_nanf("") : __builtin_bit_cast(float, e << 23);
+    return emu_bf16x2{(__bf16)(f[0] * s), (__bf16)(f[1] * s)};
+}
+// v_perm_b32: byte k of the result is byte sel[k] of {b (0..3), a (4..7)}
+static inline unsigned __builtin_amdgcn_perm(unsigned a, unsigned b, unsigned sel) {
+    const unsigned long long v = (unsigned long long)a << 32 | b;
+    unsigned r = 0;
+    for (int k = 0; k < 4; ++k) r |= (unsigned)(v >> (8 * (sel >> (8 * k) & 7)) & 0xff) << (8 * k);
+    return r;
+}
 
 // DPP: the four controls the kernels use, row_mask = bank_mask = 0xF, bound_ctrl: quad_perm [1,0,3,2] (0xB1),
 // quad_perm [2,3,0,1] (0x4E), row_half_mirror (0x141), row_mirror (0x140)
@@ -348,6 +363,16 @@ static inline emu_u32x4 __builtin_amdgcn_raw_buffer_load_b128(emu_rsrc r, unsign
     if (off + 16 <= r.num) memcpy(&v, r.base + off, 16);
     return v;
 }
+typedef unsigned emu_u32x2 __attribute__((ext_vector_type(2)));
+template <typename V> static inline V emu_raw_buffer_load(emu_rsrc r, unsigned voff, unsigned soff) {
+    const unsigned long long off = (unsigned long long)voff + soff;
+    V v{};
+    if (off + sizeof(V) <= r.num) memcpy(&v, r.base + off, sizeof(V));
+    return v;
+}
+#define __builtin_amdgcn_raw_buffer_load_b64(r, v, s, a) emu_raw_buffer_load<emu_u32x2>((r), (v), (s))
+#define __builtin_amdgcn_raw_buffer_load_b32(r, v, s, a) emu_raw_buffer_load<unsigned>((r), (v), (s))
+#define __builtin_amdgcn_raw_buffer_load_b8(r, v, s, a) emu_raw_buffer_load<unsigned char>((r), (v), (s))
 // LDS-DMA (`buffer_load_dwordx4 ... offen lds` with m0 = LDS base): lane l's 16 bytes land at LDS[m0 + 16 l]
 static inline void emu_buffer_load_lds16(emu_rsrc r, unsigned voff, unsigned soff, unsigned lds_addr) {
     const emu_u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(r, voff, soff, 0);

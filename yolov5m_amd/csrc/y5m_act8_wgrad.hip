@@ -5,21 +5,23 @@
 // and in f32 (24 bits) of three bf16 values. Products of bf16 MFMAs are exact in f32, so every type runs on the bf16 matrix cores
 // with f32 accumulation, and nothing is rounded before the sum (f32 MFMA: 1/16 of the rate).
 //
-// A workgroup (4 waves) owns a 128 x 128 tile of dW and a range of rows; per step 64 rows of dY and of the codes go through registers
-// (the codes become bf16 there) into LDS as [32 rows][16 channels] sub-tiles, and the fragments come back through
-// ds_read_b64_tr_b16, which transposes 4 x 16 blocks: 4 rows of one channel per lane. Row ranges are joined from f32 partial tiles by
-// a second launch in a fixed order (no atomics: one result per input).
+// An MFMA operand wants 8 consecutive k (rows) of ONE channel per lane, memory has 8 channels of one row next to each other. No LDS
+// is needed for that transpose: the order of rows and channels inside a tile is free as long as both operands agree on the rows. Lane
+// (i = lane & 15, g = lane >> 4) loads rows 8 g .. 8 g + 7 of its OWN P channels (16 bytes of bf16, 8 of codes: a 16-lane group reads
+// 256 consecutive bytes of a row), and byte permutes (one per two values) turn the 8 x P block into P operands. Operand ja of lane i is
+// then channel P i + ja: the product of operands (ja, jb) is the 16 x 16 block of dW at rows P i + ja, columns P i' + jb, and the P x P
+// products of one 32-row step fill a (16 P)^2 tile: 128 x 128, 64 MFMAs, 256 accumulators a lane, one wave per SIMD, no barrier in the loop.
+// A lane ends up with P consecutive columns of a row of dW: 16-byte stores.
+// The four waves of a workgroup are WN x WC tiles side by side (they share operands through L1) times WK interleaved parts of the
+// rows, added in LDS; row ranges of different workgroups are joined from f32 partial tiles by a second launch in a fixed order (no
+// atomics: one result per input).
 #include "y5m_act8.h"
 
 #define AW_THREADS 256
-#define AW_T 128                  // tile edge (channels of dY, channels of X)
-#define AW_K 64                   // rows per step
-#define AW_SUB 1088               // [32][16] bf16 sub-tile: 1024 bytes + 64 so that neighbouring sub-tiles start on other banks
-#define AW_TILE ((AW_K / 32) * (AW_T / 16) * AW_SUB)
+#define AW_K 32                   // rows per step of a wave
 
 typedef __bf16 aw_bf16x8 __attribute__((ext_vector_type(8)));
 typedef float aw_f32x4 __attribute__((ext_vector_type(4)));
-typedef short aw_s16x4 __attribute__((ext_vector_type(4)));
 
 struct AwParams {
     const void* dy;
@@ -27,185 +29,391 @@ struct AwParams {
     float *part, *dbpart;          // [ranges][N][C], [ranges][N]
     float *dw, *db;
     int64_t M, S, dn, dr;
-    int N, C, ldq, CB, tiles_n, tiles_c, ranges;
+    int N, C, ldq, CB, tiles_n, tiles_c, ranges, slots;
     int64_t per;                   // rows per range, a multiple of AW_K
 };
 
-__device__ __forceinline__ aw_s16x4 aw_tr(const unsigned char* sub, int lane_off, int rowblk) {
-    const unsigned char* p = sub + lane_off + rowblk * 512;
-    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((aw_s16x4 __attribute__((address_space(3)))*)(p));
-}
-__device__ __forceinline__ aw_bf16x8 aw_frag(const unsigned char* sub, int lane_off) {
-    const aw_s16x4 lo = aw_tr(sub, lane_off, 0), hi = aw_tr(sub, lane_off, 1);
-    const uint4 v = make_uint4(((const unsigned*)&lo)[0], ((const unsigned*)&lo)[1], ((const unsigned*)&hi)[0], ((const unsigned*)&hi)[1]);
-    return __builtin_bit_cast(aw_bf16x8, v);
-}
-// byte offset of the 8-channel piece pc of row r inside a tile
-__device__ __forceinline__ int aw_off(int r, int pc) {
-    return ((r >> 5) * (AW_T / 16) + (pc >> 1)) * AW_SUB + (r & 31) * 32 + (pc & 1) * 16;
-}
-
 template <int DT> struct AwPieces { static constexpr int n = DT == Y5M_BF16 ? 1 : DT == Y5M_F16 ? 2 : 3; };
-// dY values as NP bf16 summands, highest first; the last one takes what is left (exact: 8 bits each)
-template <int DT, int NP> __device__ __forceinline__ void aw_split(const Raw8<DT>& raw, act8_u32x4 out[NP]) {
-    if constexpr (NP == 1) {
-        out[0] = raw.r[0];
+
+// one step's data of a lane: 8 rows of PA channels of dY (raw) and of PC codes, and the rows' scales
+template <int DT, int PA, int PC> struct AwStage {
+    static constexpr int AD = DT == Y5M_F32 ? PA : PA / 2;
+    unsigned a[8][AD];
+    unsigned q[8][PC / 4];
+    unsigned s[8];
+};
+
+// n dwords at byte offset `off` of a buffer resource: zero beyond its last byte, in hardware
+template <int ND> __device__ __forceinline__ void aw_buffer(__amdgpu_buffer_rsrc_t rs, unsigned off, unsigned* d) {
+    if constexpr (ND == 1) {
+        d[0] = __builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, 0);
+    } else if constexpr (ND == 2) {
+        const act8_u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(rs, off, 0, 0);
+        d[0] = v[0];
+        d[1] = v[1];
     } else {
-        float v[8];
-        unpack8<DT>(raw, v);
-#pragma unroll
-        for (int p = 0; p < NP; ++p)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const uint32_t w = f32x2_to_bf16x2(v[2 * k], v[2 * k + 1]);
-                out[p][k] = w;
-                if (p + 1 < NP) {
-                    v[2 * k] -= __uint_as_float(w << 16);
-                    v[2 * k + 1] -= __uint_as_float(w & 0xffff0000u);
-                }
-            }
+        const act8_u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(rs, off, 0, 0);
+        d[0] = v[0];
+        d[1] = v[1];
+        d[2] = v[2];
+        d[3] = v[3];
+        if constexpr (ND == 8) aw_buffer<4>(rs, off + 16, d + 4);
     }
 }
 
-template <int DT, int FMT, bool AL>
-__global__ __launch_bounds__(AW_THREADS) void act8_wgrad_kernel(const AwParams P) {
+// FAST: rows at one distance, read in whole pieces through buffer resources that end with the range (the launcher keeps a range below
+// 2 GiB): rows beyond the range and channels beyond the last read as zero, the loop has no tail. Else element by element, any strides.
+template <int DT, int PA, int PC, bool FAST> struct AwLoader {
     typedef typename RowElem<DT>::T T;
+    static constexpr unsigned OOB = 0x80000000u;
+    const AwParams& P;
+    int64_t m0, m1;
+    int n, c, g;
+    bool nin, cin;
+    __amdgpu_buffer_rsrc_t ry, rq, rs;
+    unsigned ao, qo, so, as;                 // byte offsets of row 8 g of the range, bytes from row to row of dY
+    __device__ __forceinline__ AwLoader(const AwParams& P_, int64_t m0_, int64_t m1_, int n_, int c_, int g_) : P(P_), m0(m0_), m1(m1_), n(n_), c(c_), g(g_) {
+        nin = n < P.N;
+        cin = c < P.C;
+        if constexpr (FAST) {
+            as = (unsigned)(P.dr * (int64_t)sizeof(T));
+            const unsigned rows = (unsigned)(m1 - m0);
+            ry = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(static_cast<const T*>(P.dy) + m0 * P.dr), 0, (rows - 1) * as + (unsigned)P.N * (unsigned)sizeof(T), 0x00020000);
+            rq = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(P.q + m0 * P.ldq), 0, rows * (unsigned)P.ldq, 0x00020000);
+            rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(P.scale + m0 * P.CB), 0, rows * (unsigned)P.CB, 0x00020000);
+            ao = nin ? (unsigned)(8 * g) * as + (unsigned)n * (unsigned)sizeof(T) : OOB;
+            qo = cin ? (unsigned)(8 * g) * (unsigned)P.ldq + (unsigned)c : OOB;
+            so = cin ? (unsigned)(8 * g) * (unsigned)P.CB + ((unsigned)c >> 5) : OOB;
+        }
+    }
+    __device__ __forceinline__ void load(AwStage<DT, PA, PC>& st, unsigned step) const {       // step: rows from m0
+        constexpr int AD = AwStage<DT, PA, PC>::AD;
+        if constexpr (FAST) {
+            const unsigned a = ao + step * as, q = qo + step * (unsigned)P.ldq, s = so + step * (unsigned)P.CB;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                aw_buffer<AD>(ry, a + (unsigned)j * as, st.a[j]);
+                aw_buffer<PC / 4>(rq, q + (unsigned)(j * P.ldq), st.q[j]);
+                st.s[j] = __builtin_amdgcn_raw_buffer_load_b8(rs, s + (unsigned)(j * P.CB), 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int64_t row = m0 + step + 8 * g + j;
+                const bool in = row < m1;
+                const int64_t nb = in ? row / P.S : 0;
+                const T* p = static_cast<const T*>(P.dy) + nb * P.dn + (row - nb * P.S) * P.dr + n;
+                if constexpr (DT == Y5M_F32) {
+#pragma unroll
+                    for (int k = 0; k < PA; ++k) st.a[j][k] = in && n + k < P.N ? __float_as_uint(p[k]) : 0u;
+                } else {
+#pragma unroll
+                    for (int k = 0; k < PA / 2; ++k) {
+                        const unsigned lo = in && n + 2 * k < P.N ? p[2 * k] : 0u, hi = in && n + 2 * k + 1 < P.N ? p[2 * k + 1] : 0u;
+                        st.a[j][k] = lo | (hi << 16);
+                    }
+                }
+                const uint8_t* q = P.q + row * P.ldq + c;
+#pragma unroll
+                for (int k = 0; k < PC / 4; ++k) st.q[j][k] = in && cin ? *reinterpret_cast<const unsigned*>(q + 4 * k) : 0u;
+                st.s[j] = in && cin ? P.scale[row * P.CB + (c >> 5)] : 0u;
+            }
+        }
+    }
+};
+
+// low or high halves of two dwords: [lo.h, hi.h]
+__device__ __forceinline__ unsigned aw_pair(unsigned lo, unsigned hi, int h) {
+    return __builtin_amdgcn_perm(hi, lo, h ? 0x07060302u : 0x05040100u);
+}
+// two codes (bytes 2 h, 2 h + 1 of w) times their scale as a pair of bf16 (exact)
+template <int FMT> __device__ __forceinline__ unsigned aw_decode2(unsigned w, float scale, int h) {
+    if constexpr (FMT == Y5M_KEEP_E4M3) {
+        return __builtin_bit_cast(unsigned, h ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false));
+    } else {
+        // bytes + 128 convert in one instruction each; (b - 128) * scale as one fma, exact
+        const unsigned u = w ^ 0x80808080u;
+        const float off = -128.0f * scale;
+        return f32x2_to_bf16x2(fmaf((float)((u >> (16 * h)) & 0xffu), scale, off), fmaf((float)((u >> (16 * h + 8)) & 0xffu), scale, off));
+    }
+}
+
+template <int DT, int FMT, int PA, int PC, int WN, int WC, int WK, bool FAST, bool DB>
+__global__ __launch_bounds__(AW_THREADS, PA * PC <= 32 ? 2 : 1) void act8_wgrad_kernel(const AwParams P) {
+    static_assert(WN * WC * WK == AW_THREADS / 64, "four waves");
     constexpr int NP = AwPieces<DT>::n;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    unsigned char* Xs = smem + NP * AW_TILE;
-    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, wn = wid & 1, wc = wid >> 1;
-    unsigned b = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, i16 = lane & 15, g = lane >> 4;
+    const int wn = wid % WN, wc = (wid / WN) % WC, wk = wid / (WN * WC);
+    // workgroups go round the 8 XCDs: give each XCD a contiguous stretch of the range-major order, so that the tiles that read the
+    // same rows share its L2
+    const unsigned q8 = gridDim.x >> 3, r8 = gridDim.x & 7, xcd = blockIdx.x & 7;
+    unsigned b = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + (blockIdx.x >> 3);
     const int ct = (int)(b % (unsigned)P.tiles_c);
     b /= (unsigned)P.tiles_c;
     const int nt = (int)(b % (unsigned)P.tiles_n), range = (int)(b / (unsigned)P.tiles_n);
-    const int n0 = nt * AW_T, c0 = ct * AW_T;
+    const int n0 = (nt * WN + wn) * 16 * PA, c0 = (ct * WC + wc) * 16 * PC;
     const int64_t m0 = range * P.per, m1 = m0 + P.per < P.M ? m0 + P.per : P.M;
 
-    aw_f32x4 acc[4][4];
+    aw_f32x4 acc[PA][PC];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < PA; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = (aw_f32x4){0.f, 0.f, 0.f, 0.f};
-    float bias[8];
+        for (int j = 0; j < PC; ++j) acc[i][j] = (aw_f32x4){0.f, 0.f, 0.f, 0.f};
+    float bias[PA];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) bias[k] = 0.f;
-    const bool want_db = P.dbpart && ct == 0;
+    for (int k = 0; k < PA; ++k) bias[k] = 0.f;
 
-    // loader: 16 threads per row (8 channels each), 16 rows at once, 4 times
-    const int pc = tid & 15, rl = tid >> 4;
-    const int yc = n0 + pc * 8, xc = c0 + pc * 8;
-    const bool yin = yc < P.N, xin = xc < P.C;
-    const int lane_off = (4 * (lane >> 4) + ((lane & 15) >> 2)) * 32 + (lane & 3) * 8;
-
-    for (int64_t m = m0; m < m1; m += AW_K) {
-        __syncthreads();
+    const AwLoader<DT, PA, PC, FAST> L(P, m0, m1, n0 + PA * i16, c0 + PC * i16, g);
+    auto compute = [&](AwStage<DT, PA, PC>& st) __attribute__((always_inline)) {
+        // (rows and channels beyond the last: codes 0, scale byte 0 = 0.0)
+        aw_bf16x8 xf[PC];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int r = u * 16 + rl;
-            const int64_t row = m + r;
-            Raw8<DT> y = {};
-            act8_u32x2 q = {0u, 0u};
-            float sc = 1.0f;
-            if (row < m1) {
-                const int64_t n = row / P.S;
-                if (yin) y = load_raw8<DT, AL>(static_cast<const T*>(P.dy) + n * P.dn + (row - n * P.S) * P.dr + yc, P.N - yc);
-                if (xin) {
-                    q = *reinterpret_cast<const act8_u32x2*>(P.q + row * P.ldq + xc);
-                    sc = act8_scale(P.scale[row * P.CB + (xc >> 5)]);
-                }
-            }
-            act8_u32x4 yp[NP];
-            aw_split<DT, NP>(y, yp);
+        for (int w = 0; w < PC / 2; ++w) {
+            unsigned v[8];
 #pragma unroll
-            for (int p = 0; p < NP; ++p) *reinterpret_cast<act8_u32x4*>(smem + p * AW_TILE + aw_off(r, pc)) = yp[p];
-            if (want_db) {
-                float v[8];
-                unpack8<DT>(y, v);
+            for (int j = 0; j < 8; ++j) v[j] = aw_decode2<FMT>(st.q[j][w >> 1], act8_scale(st.s[j]), w & 1);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) bias[k] += v[k];
-            }
-            float xv[8];
-            act8_decode8<FMT>(q, sc, xv);
-            act8_u32x4 xp;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) xp[k] = f32x2_to_bf16x2(xv[2 * k], xv[2 * k + 1]);
-            *reinterpret_cast<act8_u32x4*>(Xs + aw_off(r, pc)) = xp;
+            for (int h = 0; h < 2; ++h)
+                xf[2 * w + h] = __builtin_bit_cast(aw_bf16x8, (act8_u32x4){aw_pair(v[0], v[1], h), aw_pair(v[2], v[3], h), aw_pair(v[4], v[5], h), aw_pair(v[6], v[7], h)});
         }
-        __syncthreads();
 #pragma unroll
-        for (int ks = 0; ks < AW_K / 32; ++ks) {
-            aw_bf16x8 xf[4];
+        for (int ja = 0; ja < PA; ++ja) {
+            act8_u32x4 yf[NP];
+            if constexpr (DT == Y5M_BF16) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) xf[j] = aw_frag(Xs + (ks * (AW_T / 16) + wc * 4 + j) * AW_SUB, lane_off);
+                for (int p = 0; p < 4; ++p) yf[0][p] = aw_pair(st.a[2 * p][ja >> 1], st.a[2 * p + 1][ja >> 1], ja & 1);
+                if constexpr (DB) {
 #pragma unroll
-            for (int p = 0; p < NP; ++p)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const aw_bf16x8 yf = aw_frag(smem + p * AW_TILE + (ks * (AW_T / 16) + wn * 4 + i) * AW_SUB, lane_off);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(yf, xf[j], acc[i][j], 0, 0, 0);
+                    for (int p = 0; p < 4; ++p) bias[ja] += __uint_as_float(yf[0][p] << 16) + __uint_as_float(yf[0][p] & 0xffff0000u);
                 }
+            } else {
+                // the value as a sum of NP bf16, highest first; what is left after the others fits the last one
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    float lo, hi;
+                    if constexpr (DT == Y5M_F32) {
+                        lo = __uint_as_float(st.a[2 * p][ja]);
+                        hi = __uint_as_float(st.a[2 * p + 1][ja]);
+                    } else {
+                        lo = f16_to_f32((uint16_t)(st.a[2 * p][ja >> 1] >> (16 * (ja & 1))));
+                        hi = f16_to_f32((uint16_t)(st.a[2 * p + 1][ja >> 1] >> (16 * (ja & 1))));
+                    }
+                    if constexpr (DB) bias[ja] += lo + hi;
+#pragma unroll
+                    for (int e = 0; e < NP; ++e) {
+                        const unsigned w = f32x2_to_bf16x2(lo, hi);
+                        yf[e][p] = w;
+                        lo -= __uint_as_float(w << 16);
+                        hi -= __uint_as_float(w & 0xffff0000u);
+                    }
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < NP; ++e)
+#pragma unroll
+                for (int jb = 0; jb < PC; ++jb)
+                    acc[ja][jb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(aw_bf16x8, yf[e]), xf[jb], acc[ja][jb], 0, 0, 0);
+        }
+    };
+
+    // this wave's steps are rows 32 (wk + WK t) of the range; the next step's loads are in flight under the current one's products.
+    // Steps are taken in pairs: one beyond the end reads zeros.
+    const unsigned rows = (unsigned)(m1 - m0), stride = AW_K * WK;
+    AwStage<DT, PA, PC> s0, s1;
+    L.load(s0, AW_K * wk);
+    for (unsigned t = AW_K * wk; t < rows; t += 2 * stride) {
+        // (the loads stay ahead of the products: left to itself the scheduler sinks each to its use and waits for it there)
+        L.load(s1, t + stride);
+        __builtin_amdgcn_sched_barrier(0);
+        compute(s0);
+        __builtin_amdgcn_sched_barrier(0);
+        L.load(s0, t + 2 * stride);
+        __builtin_amdgcn_sched_barrier(0);
+        compute(s1);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+
+    // bias: the four row groups of the wave
+    if constexpr (DB) {
+#pragma unroll
+        for (int k = 0; k < PA; ++k) {
+            bias[k] += __shfl_xor(bias[k], 16, 64);
+            bias[k] += __shfl_xor(bias[k], 32, 64);
         }
     }
-    // D[n][c]: lane holds n = 4 (lane >> 4) + r, c = lane & 15
-    float* part = P.part + (size_t)range * P.N * P.C;
+    // the WK parts of a tile are added in LDS, PA / 2 operands' worth at a time
+    constexpr int HALF = PA / 2 * PC * 4;                      // floats of a lane
+    float* red = reinterpret_cast<float*>(smem);               // [WK - 1][WN * WC][HALF][64], then [WK][WN][16 PA]
+    float* redb = red + (WK > 1 ? (size_t)(WK - 1) * WN * WC * HALF * 64 : 0);
+    if constexpr (WK > 1) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+        for (int half = 0; half < 2; ++half) {
+            __syncthreads();
+            if (wk > 0) {
+                float* d = red + ((size_t)(wk - 1) * WN * WC + wid % (WN * WC)) * HALF * 64 + lane;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int c = c0 + (wc * 4 + j) * 16 + (lane & 15);
+                for (int i = 0; i < PA / 2; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int n = n0 + (wn * 4 + i) * 16 + 4 * (lane >> 4) + r;
-                if (n < P.N && c < P.C) part[(size_t)n * P.C + c] = acc[i][j][r];
+                    for (int j = 0; j < PC; ++j)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) d[((i * PC + j) * 4 + r) * 64] = acc[half * (PA / 2) + i][j][r];
+            }
+            __syncthreads();
+            if (wk == 0) {
+#pragma unroll
+                for (int o = 1; o < WK; ++o) {
+                    const float* d = red + ((size_t)(o - 1) * WN * WC + wid % (WN * WC)) * HALF * 64 + lane;
+#pragma unroll
+                    for (int i = 0; i < PA / 2; ++i)
+#pragma unroll
+                        for (int j = 0; j < PC; ++j)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) acc[half * (PA / 2) + i][j][r] += d[((i * PC + j) * 4 + r) * 64];
+                }
             }
         }
-    if (P.dbpart) {                                            // (uniform over the launch)
-        float* red = reinterpret_cast<float*>(smem);
+    }
+    if constexpr (DB) {
         __syncthreads();
+        if (ct == 0 && wc == 0 && g == 0) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) red[rl * AW_T + pc * 8 + k] = bias[k];
+            for (int k = 0; k < PA; ++k) redb[(wk * WN + wn) * 16 * PA + PA * i16 + k] = bias[k];
+        }
         __syncthreads();
-        if (want_db && tid < AW_T && n0 + tid < P.N) {
+        const int nn = nt * WN * 16 * PA + tid;
+        if (ct == 0 && tid < WN * 16 * PA && nn < P.N) {
             float t = 0.f;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) t += red[r * AW_T + tid];
-            P.dbpart[(size_t)range * P.N + n0 + tid] = t;
+            for (int o = 0; o < WK; ++o) t += redb[o * WN * 16 * PA + tid];
+            P.dbpart[(size_t)range * P.N + nn] = t;
         }
     }
-}
-
-// dW = sum of the ranges' tiles, in order
-__global__ __launch_bounds__(AW_THREADS) void act8_wgrad_join_kernel(const AwParams P) {
-    const int64_t i = (int64_t)blockIdx.x * AW_THREADS + threadIdx.x, nw = (int64_t)P.N * P.C;
-    if (i < nw) {
-        double t = 0.0;
-        for (int r = 0; r < P.ranges; ++r) t += (double)P.part[(size_t)r * nw + i];
-        P.dw[i] = (float)t;
-    } else if (P.db && i - nw < P.N) {
-        double t = 0.0;
-        for (int r = 0; r < P.ranges; ++r) t += (double)P.dbpart[(size_t)r * P.N + (i - nw)];
-        P.db[i - nw] = (float)t;
+    if (wk == 0) {
+        // lane: rows n0 + PA (4 g + r) + ja, columns c0 + PC i16 .. + PC - 1
+        float* part = P.part + (size_t)range * P.N * P.C;
+        const int c = c0 + PC * i16;
+        const bool vec = (P.C & 3) == 0;
+#pragma unroll
+        for (int ja = 0; ja < PA; ++ja)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int n = n0 + PA * (4 * g + r) + ja;
+                if (n >= P.N) continue;
+                float* d = part + (size_t)n * P.C + c;
+#pragma unroll
+                for (int h = 0; h < PC / 4; ++h) {
+                    if (vec && c + 4 * h < P.C) {
+                        *reinterpret_cast<aw_f32x4*>(d + 4 * h) = (aw_f32x4){acc[ja][4 * h][r], acc[ja][4 * h + 1][r], acc[ja][4 * h + 2][r], acc[ja][4 * h + 3][r]};
+                    } else if (!vec) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (c + 4 * h + k < P.C) d[4 * h + k] = acc[ja][4 * h + k][r];
+                    }
+                }
+            }
     }
 }
 
-static void aw_geometry(AwParams& P, int64_t M, int N, int C) {
+// dW = sum of the ranges' tiles: `slots` threads share an output, each takes every slots-th range; joined in order, in f64
+__global__ __launch_bounds__(AW_THREADS) void act8_wgrad_join_kernel(const AwParams P) {
+    __shared__ double red[AW_THREADS];
+    const int per = AW_THREADS / P.slots, o = threadIdx.x % per, slot = threadIdx.x / per;
+    const int64_t i = (int64_t)blockIdx.x * per + o, nw = (int64_t)P.N * P.C;
+    const bool isw = i < nw, in = isw || (P.db && i - nw < P.N);
+    const float* src = isw ? P.part + i : P.dbpart + (i - nw);
+    const size_t step = isw ? (size_t)nw : (size_t)P.N;
+    double t = 0.0;
+    if (in) {
+        int r = slot;
+        for (; r + 7 * P.slots < P.ranges; r += 8 * P.slots) {
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = src[(size_t)(r + u * P.slots) * step];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) t += (double)v[u];
+        }
+        for (; r < P.ranges; r += P.slots) t += (double)src[(size_t)r * step];
+    }
+    if (P.slots > 1) {
+        red[threadIdx.x] = t;
+        __syncthreads();
+        if (slot != 0) return;
+        t = 0.0;
+        for (int s = 0; s < P.slots; ++s) t += red[s * per + o];
+    }
+    if (in) (isw ? P.dw : P.db)[isw ? i : i - nw] = (float)t;
+}
+
+// Tiles. bf16 in whole pieces: an edge of 128, or 64 where the weight is no wider (half the wasted products). fp16 / f32 (two or three
+// products per value, twice the raw registers) and rows read element by element: 64 x 64, two waves per SIMD. Waves: two tiles of dY
+// channels (else of X channels) side by side where there are two, so that a workgroup's partial tiles are joined in LDS only twice;
+// else all four waves split the rows of one tile.
+struct AwShape { int pa, pc, wn, wc, wk; };
+static AwShape aw_shape(int N, int C, bool wide) {
+    AwShape s;
+    s.pa = !wide || N <= 64 ? 4 : 8;
+    s.pc = !wide || C <= 64 ? 4 : 8;
+    const int tn = (N + 16 * s.pa - 1) / (16 * s.pa), tc = (C + 16 * s.pc - 1) / (16 * s.pc);
+    s.wn = s.pa == 8 && s.pc == 8 && tn % 2 == 0 ? 2 : 1;
+    s.wc = s.pa == 8 && s.pc == 8 && s.wn == 1 && tc % 2 == 0 ? 2 : 1;
+    s.wk = 4 / (s.wn * s.wc);
+    return s;
+}
+static void aw_geometry(AwParams& P, const AwShape& s, int64_t M, int N, int C) {
     P.M = M; P.N = N; P.C = C; P.CB = (C + 31) / 32;
-    P.tiles_n = (N + AW_T - 1) / AW_T;
-    P.tiles_c = (C + AW_T - 1) / AW_T;
-    const int64_t tiles = (int64_t)P.tiles_n * P.tiles_c, steps = (M + AW_K - 1) / AW_K;
-    int64_t want = (1024 + tiles - 1) / tiles, most = (steps + 3) / 4;     // about 4 workgroups per CU, at least 4 steps each
+    P.tiles_n = (N + 16 * s.pa * s.wn - 1) / (16 * s.pa * s.wn);
+    P.tiles_c = (C + 16 * s.pc * s.wc - 1) / (16 * s.pc * s.wc);
+    // ranges: as many workgroups as fit the CUs at once (two per CU below 128 x 128), at least 4 steps per wave, and less than
+    // 2 GiB of rows each
+    const int64_t tiles = (int64_t)P.tiles_n * P.tiles_c, steps = (M + AW_K - 1) / AW_K, most = (steps + 4 * s.wk - 1) / (4 * s.wk);
+    int64_t want = (s.pa * s.pc <= 32 ? 512 : 256) / tiles;
     if (want > most) want = most;
     if (want < 1) want = 1;
-    P.per = (steps + want - 1) / want * AW_K;
+    int64_t per = (steps + want - 1) / want * AW_K;
+    const int64_t cap = (1ll << 30) / (4ll * (N > C + 8 ? N : C + 8)) / AW_K * AW_K;
+    if (per > cap) per = cap > AW_K ? cap : AW_K;
+    P.per = per;
     P.ranges = (int)((M + P.per - 1) / P.per);
+    P.slots = P.ranges > 64 ? 16 : P.ranges > 16 ? 4 : 1;
 }
 
 extern "C" size_t y5m_act8_wgrad_workspace_bytes(int64_t M, int Cout, int C) {
     if (M <= 0 || Cout <= 0 || C <= 0) return 0;
     AwParams P = {};
-    aw_geometry(P, M, Cout, C);
-    return (size_t)P.ranges * ((size_t)Cout * C + Cout) * sizeof(float);
+    aw_geometry(P, aw_shape(Cout, C, true), M, Cout, C);
+    const int a = P.ranges;
+    aw_geometry(P, aw_shape(Cout, C, false), M, Cout, C);
+    return (size_t)(a > P.ranges ? a : P.ranges) * ((size_t)Cout * C + Cout) * sizeof(float);
+}
+
+template <int DT, int FMT, int PA, int PC, int WN, int WC, bool FAST, bool DB>
+static int aw_launch_db(const AwParams& P, hipStream_t st) {
+    constexpr int WK = 4 / (WN * WC), lds = ((WK - 1) * WN * WC * (PA / 2 * PC * 4) * 64 + WK * WN * 16 * PA) * (int)sizeof(float);
+    static_assert(lds <= 160 * 1024, "LDS");
+    if constexpr (lds > 64 * 1024) {
+        static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(act8_wgrad_kernel<DT, FMT, PA, PC, WN, WC, WK, FAST, DB>),
+                                                        hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) { y5m_set_error("act8_wgrad_kernel: %d bytes of LDS refused", lds); return Y5M_ELAUNCH; }
+    }
+    hipLaunchKernelGGL((act8_wgrad_kernel<DT, FMT, PA, PC, WN, WC, WK, FAST, DB>), dim3((unsigned)((int64_t)P.tiles_n * P.tiles_c * P.ranges)), dim3(AW_THREADS), lds, st, P);
+    Y5M_CHECK_LAUNCH("act8_wgrad_kernel");
+    return Y5M_OK;
+}
+template <int DT, int FMT, int PA, int PC, int WN, int WC, bool FAST> static int aw_launch(const AwParams& P, hipStream_t st) {
+    return P.dbpart ? aw_launch_db<DT, FMT, PA, PC, WN, WC, FAST, true>(P, st) : aw_launch_db<DT, FMT, PA, PC, WN, WC, FAST, false>(P, st);
+}
+template <int FMT> static int aw_dispatch(const AwParams& P, const AwShape& s, int dtype, bool fast, hipStream_t st) {
+    constexpr int B = Y5M_BF16, H = Y5M_F16, F = Y5M_F32;
+    if (s.pa == 4 && s.pc == 4) {
+        if (dtype == F) return fast ? aw_launch<F, FMT, 4, 4, 1, 1, true>(P, st) : aw_launch<F, FMT, 4, 4, 1, 1, false>(P, st);
+        if (dtype == H) return fast ? aw_launch<H, FMT, 4, 4, 1, 1, true>(P, st) : aw_launch<H, FMT, 4, 4, 1, 1, false>(P, st);
+        return fast ? aw_launch<B, FMT, 4, 4, 1, 1, true>(P, st) : aw_launch<B, FMT, 4, 4, 1, 1, false>(P, st);
+    }
+    if (s.pa == 4) return aw_launch<B, FMT, 4, 8, 1, 1, true>(P, st);
+    if (s.pc == 4) return aw_launch<B, FMT, 8, 4, 1, 1, true>(P, st);
+    if (s.wn == 2) return aw_launch<B, FMT, 8, 8, 2, 1, true>(P, st);
+    return s.wc == 2 ? aw_launch<B, FMT, 8, 8, 1, 2, true>(P, st) : aw_launch<B, FMT, 8, 8, 1, 1, true>(P, st);
 }
 
 extern "C" int y5m_act8_wgrad(const void* dy, int64_t dy_batch_stride, int64_t dy_row_stride, int64_t N, int64_t S, int Cout, const void* q, int ldq,
@@ -220,42 +428,30 @@ extern "C" int y5m_act8_wgrad(const void* dy, int64_t dy_batch_stride, int64_t d
         return rc != Y5M_OK || !db ? rc : y5m_fill32(db, 0, Cout, y5m_stream(stream));
     }
     Y5M_REQUIRE(dy && q && scale, "null pointer");
-    Y5M_REQUIRE(ldq >= C && ldq % 8 == 0 && ((uintptr_t)q & 7) == 0, "8-bit form: ldq % 8 == 0, at least C, codes 8-byte aligned");
-    Y5M_REQUIRE(ws && ws_bytes >= y5m_act8_wgrad_workspace_bytes(N * S, Cout, C), "workspace too small");
+    Y5M_REQUIRE(ldq >= C && ldq % 8 == 0 && ldq <= (1 << 26) && ((uintptr_t)q & 7) == 0, "8-bit form: ldq % 8 == 0, at least C, codes 8-byte aligned");
+    Y5M_REQUIRE(((uintptr_t)ws & 15) == 0 && ws && ws_bytes >= y5m_act8_wgrad_workspace_bytes(N * S, Cout, C), "workspace too small or not 16-byte aligned");
+    // rows of all samples at one distance in whole vector pieces, and a range of them within a buffer resource's 32-bit offsets
+    const int64_t pitch = S == 1 && N > 1 ? dy_batch_stride : dy_row_stride;      // (one row per sample: the samples are the rows)
+    bool fast = rows_aligned16(dy, dy_batch_stride, dy_row_stride, N, S, Cout, dtype) && (N == 1 || S == 1 || dy_batch_stride == S * dy_row_stride) &&
+                pitch >= Cout && pitch < (1 << 24);
     AwParams P = {};
-    aw_geometry(P, N * S, Cout, C);
-    P.dy = dy; P.dn = dy_batch_stride; P.dr = dy_row_stride; P.S = S;
+    AwShape s = aw_shape(Cout, C, fast && dtype == Y5M_BF16);
+    aw_geometry(P, s, N * S, Cout, C);
+    if (fast && (P.per + 4 * AW_K * s.wk) * (pitch > ldq ? pitch : ldq) * (dtype == Y5M_F32 ? 4 : 2) >= (1ll << 31)) {
+        fast = false;
+        s = aw_shape(Cout, C, false);
+        aw_geometry(P, s, N * S, Cout, C);
+    }
+    P.dy = dy; P.dn = dy_batch_stride; P.dr = fast ? pitch : dy_row_stride; P.S = S;
     P.q = static_cast<const uint8_t*>(q); P.scale = static_cast<const uint8_t*>(scale); P.ldq = ldq;
     P.part = static_cast<float*>(ws);
     P.dbpart = db ? P.part + (size_t)P.ranges * Cout * C : nullptr;
     P.dw = dw; P.db = db;
-    const int64_t blocks = (int64_t)P.tiles_n * P.tiles_c * P.ranges;
-    Y5M_REQUIRE(blocks < (1ll << 31), "too many workgroups");
-    const bool al = rows_aligned16(dy, dy_batch_stride, dy_row_stride, N, S, Cout, dtype);
-#define GO(DT, FMT, AL)                                                                                                          \
-    do {                                                                                                                         \
-        constexpr int lds = (AwPieces<DT>::n + 1) * AW_TILE;                                                                     \
-        static bool set = false;                                                                                                 \
-        if (!set && hipFuncSetAttribute(reinterpret_cast<const void*>(act8_wgrad_kernel<DT, FMT, AL>), hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) { \
-            y5m_set_error("act8_wgrad_kernel: %d bytes of LDS refused", lds);                                                    \
-            return Y5M_ELAUNCH;                                                                                                  \
-        }                                                                                                                        \
-        set = true;                                                                                                              \
-        hipLaunchKernelGGL((act8_wgrad_kernel<DT, FMT, AL>), dim3((unsigned)blocks), dim3(AW_THREADS), lds, y5m_stream(stream), P); \
-    } while (0)
-#define GO2(DT)                                                                                                                  \
-    do {                                                                                                                         \
-        if (fmt == Y5M_KEEP_E4M3) { if (al) GO(DT, Y5M_KEEP_E4M3, true); else GO(DT, Y5M_KEEP_E4M3, false); }                    \
-        else { if (al) GO(DT, Y5M_KEEP_INT8, true); else GO(DT, Y5M_KEEP_INT8, false); }                                         \
-    } while (0)
-    if (dtype == Y5M_F32) GO2(Y5M_F32);
-    else if (dtype == Y5M_BF16) GO2(Y5M_BF16);
-    else GO2(Y5M_F16);
-#undef GO2
-#undef GO
-    Y5M_CHECK_LAUNCH("act8_wgrad_kernel");
-    const int64_t items = (int64_t)Cout * C + (db ? Cout : 0);
-    hipLaunchKernelGGL(act8_wgrad_join_kernel, dim3((unsigned)((items + AW_THREADS - 1) / AW_THREADS)), dim3(AW_THREADS), 0, y5m_stream(stream), P);
+    Y5M_REQUIRE((int64_t)P.tiles_n * P.tiles_c * P.ranges < (1ll << 31), "too many workgroups");
+    const int rc = fmt == Y5M_KEEP_E4M3 ? aw_dispatch<Y5M_KEEP_E4M3>(P, s, dtype, fast, y5m_stream(stream)) : aw_dispatch<Y5M_KEEP_INT8>(P, s, dtype, fast, y5m_stream(stream));
+    if (rc != Y5M_OK) return rc;
+    const int64_t items = (int64_t)Cout * C + (db ? Cout : 0), per = AW_THREADS / P.slots;
+    hipLaunchKernelGGL(act8_wgrad_join_kernel, dim3((unsigned)((items + per - 1) / per)), dim3(AW_THREADS), 0, y5m_stream(stream), P);
     Y5M_CHECK_LAUNCH("act8_wgrad_join_kernel");
     return Y5M_OK;
 }
