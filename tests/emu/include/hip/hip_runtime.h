@@ -102,6 +102,7 @@ static inline float __uint_as_float(unsigned u) { return __builtin_bit_cast(floa
 static inline float __int_as_float(int u) { return __builtin_bit_cast(float, u); }
 static inline unsigned __float_as_uint(float f) { return __builtin_bit_cast(unsigned, f); }
 static inline int __float_as_int(float f) { return __builtin_bit_cast(int, f); }
+static inline unsigned __umulhi(unsigned a, unsigned b) { return (unsigned)((unsigned long long)a * b >> 32); }
 static inline unsigned __umul24(unsigned a, unsigned b) { return (a & 0xffffffu) * (b & 0xffffffu); }
 static inline int __mul24(int a, int b) { return ((a << 8) >> 8) * ((b << 8) >> 8); }
 // __expf on the GPU is v_exp_f32(x * log2(e)) with the product rounded to f32 (argument error ~ |x| 6e-8 relative in the result);

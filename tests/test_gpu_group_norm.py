@@ -288,19 +288,27 @@ def test_rows_between_and_behind_the_output_are_left_alone():
             assert (t[:, s] == 7.0)[:, odd:].all() and (t[:, :s, c + odd:] == 7.0).all() and (odd == 0 or (t[0, 0, :odd] == 7.0).all())
 
 
-def test_in_place_at_the_c_entry():
+@pytest.mark.parametrize("shape", [(2, 90, 40), (1, 2000, 136)])
+def test_in_place_at_the_c_entry(shape):
+    """z over x, dx over dz"""
     import yolov5m_amd.group_norm  # noqa: F401
     from yolov5m_amd import _lib
     L = _lib.lib()
-    n, s, c, g = 2, 90, 40, 5
-    x = torch.randn(n, s, c, generator=torch.Generator().manual_seed(25)).to(DEV)
-    ref = Exact(x.clone().transpose(1, 2), g, None, None, 1e-5, "silu")
+    (n, s, c), g = shape, 4
+    x, dz = (torch.randn(n, s, c, generator=torch.Generator().manual_seed(k)).to(DEV) for k in (25, 26))
+    xt = x.clone().transpose(1, 2)
+    ref = Exact(xt, g, None, None, 1e-5, "silu", None, dz.clone().transpose(1, 2))
     stat = torch.empty(2 * n * g, device=DEV)
-    wsb = L.y5m_gn_act_workspace_bytes(n, s, c, g)
+    wsb = L.y5m_gn_act_bwd_workspace_bytes(n, s, c, g)
     ws = torch.empty(wsb, dtype=torch.uint8, device=DEV)
-    _lib.check(L.y5m_gn_act(x.data_ptr(), s * c, c, None, None, n, s, c, g, 1e-5, 1, x.data_ptr(), s * c, c, stat.data_ptr(), stat.data_ptr() + 4 * n * g,
+    keep = x.clone()
+    p = stat.data_ptr()
+    _lib.check(L.y5m_gn_act(x.data_ptr(), s * c, c, None, None, n, s, c, g, 1e-5, 1, x.data_ptr(), s * c, c, p, p + 4 * n * g,
                             None, 0, None, 0, ws.data_ptr(), wsb, 0, _lib.stream_ptr()), "y5m_gn_act")
     ref.check(x.transpose(1, 2), "z")
+    _lib.check(L.y5m_gn_act_bwd(dz.data_ptr(), s * c, c, keep.data_ptr(), s * c, c, None, 0, None, 0, None, None, p, p + 4 * n * g, n, s, c, g, 1,
+                                dz.data_ptr(), s * c, c, None, None, ws.data_ptr(), wsb, 0, _lib.stream_ptr()), "y5m_gn_act_bwd")
+    ref.check(dz.transpose(1, 2), "dx")
 
 
 def test_refusals():

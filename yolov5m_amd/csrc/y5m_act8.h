@@ -25,13 +25,17 @@ template <int DT> struct Raw8 { act8_u32x4 r[DT == Y5M_F32 ? 2 : 1]; };
 __device__ __forceinline__ float f16_to_f32(uint16_t h) { return (float)__builtin_bit_cast(y5m_f16, h); }
 __device__ __forceinline__ uint16_t f32_to_f16(float f) { return __builtin_bit_cast(uint16_t, (y5m_f16)f); }
 
-// AL: 16-byte pieces (the launcher checks base, strides and C); else element by element, channels >= nv read as 0
-template <int DT, bool AL>
+// AL = 1: 16-byte pieces (the launcher checks base, strides and C). Else pieces that start at any element (unaligned vector loads where the
+// whole piece is inside the row: at 255 f32 channels a third of the time of element loads), a row's last piece by elements, the
+// channels >= nv as 0
+template <int DT, int AL>
 __device__ __forceinline__ Raw8<DT> load_raw8(const typename RowElem<DT>::T* __restrict__ p, int nv) {
     Raw8<DT> w;
     if constexpr (AL) {
         w.r[0] = *reinterpret_cast<const act8_u32x4*>(p);
         if constexpr (DT == Y5M_F32) w.r[1] = *reinterpret_cast<const act8_u32x4*>(p + 4);
+    } else if (nv >= 8) {
+        __builtin_memcpy(&w, p, sizeof(w));
     } else if constexpr (DT == Y5M_F32) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) w.r[k >> 2][k & 3] = k < nv ? __float_as_uint(p[k]) : 0u;
@@ -52,11 +56,13 @@ template <int DT> __device__ __forceinline__ void unpack8(const Raw8<DT>& w, flo
         else v[k] = f16_to_f32((uint16_t)(w.r[0][k >> 1] >> (16 * (k & 1))));
     }
 }
-template <int DT, bool AL>
+template <int DT, int AL>
 __device__ __forceinline__ void load8(const typename RowElem<DT>::T* __restrict__ p, int nv, float v[8]) {
     unpack8<DT>(load_raw8<DT, AL>(p, nv), v);
 }
-template <int DT, bool AL>
+// AL = 2: 16-byte pieces stored past the caches. For outputs too large to be read back from the memory-side cache by whoever comes next: stored there
+// they would only push out the rows that this operator reads twice, or whose rest is still to be read
+template <int DT, int AL>
 __device__ __forceinline__ void store8(typename RowElem<DT>::T* __restrict__ p, int nv, const float v[8]) {
     Raw8<DT> w;
     if constexpr (DT == Y5M_F32) {
@@ -70,8 +76,14 @@ __device__ __forceinline__ void store8(typename RowElem<DT>::T* __restrict__ p, 
         for (int k = 0; k < 4; ++k) w.r[0][k] = (unsigned)f32_to_f16(v[2 * k]) | ((unsigned)f32_to_f16(v[2 * k + 1]) << 16);
     }
     if constexpr (AL) {
-        *reinterpret_cast<act8_u32x4*>(p) = w.r[0];
-        if constexpr (DT == Y5M_F32) *reinterpret_cast<act8_u32x4*>(p + 4) = w.r[1];
+        act8_u32x4* q = reinterpret_cast<act8_u32x4*>(p);
+#pragma unroll
+        for (int h = 0; h < (DT == Y5M_F32 ? 2 : 1); ++h) {
+            if constexpr (AL == 2) __builtin_nontemporal_store(w.r[h], q + h);
+            else q[h] = w.r[h];
+        }
+    } else if (nv >= 8) {
+        __builtin_memcpy(p, &w, sizeof(w));
     } else {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
@@ -81,6 +93,9 @@ __device__ __forceinline__ void store8(typename RowElem<DT>::T* __restrict__ p, 
             }
     }
 }
+// host: does an output of this size go past the caches? (256 MB memory-side cache; 64 x 80 x 80 x 192 in bf16, a forward and backward
+// whose outputs are 157 MB each: 226 us with, 257 without; at 79 MB 125 against 134)
+static inline bool rows_past_caches(int64_t rows, int C, int dtype) { return rows * C * (dtype == Y5M_F32 ? 4 : 2) > (64ll << 20); }
 
 // ---- the 8-bit form ---------------------------------------------------------------------------------------------------------
 template <int DT> __device__ __forceinline__ float act8_limit() {

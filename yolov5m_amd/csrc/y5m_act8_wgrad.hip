@@ -97,26 +97,39 @@ template <int DT, int PA, int PC, bool FAST> struct AwLoader {
                 st.s[j] = __builtin_amdgcn_raw_buffer_load_b8(rs, s + (unsigned)(j * P.CB), 0, 0);
             }
         } else {
+            // rows of unaligned pieces (the compiler's unaligned vector loads), a row's last piece by elements; P.S = 0: one distance
+            const bool whole = n + PA <= P.N;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int64_t row = m0 + step + 8 * g + j;
                 const bool in = row < m1;
-                const int64_t nb = in ? row / P.S : 0;
-                const T* p = static_cast<const T*>(P.dy) + nb * P.dn + (row - nb * P.S) * P.dr + n;
-                if constexpr (DT == Y5M_F32) {
+                const int64_t r = in ? row : m0, nb = P.S ? r / P.S : 0;
+                const T* p = static_cast<const T*>(P.dy) + nb * P.dn + (r - nb * P.S) * P.dr + n;
+                if (whole) {
+                    __builtin_memcpy(st.a[j], p, sizeof(st.a[j]));
+                } else if constexpr (DT == Y5M_F32) {
 #pragma unroll
-                    for (int k = 0; k < PA; ++k) st.a[j][k] = in && n + k < P.N ? __float_as_uint(p[k]) : 0u;
+                    for (int k = 0; k < PA; ++k) st.a[j][k] = n + k < P.N ? __float_as_uint(p[k]) : 0u;
                 } else {
 #pragma unroll
                     for (int k = 0; k < PA / 2; ++k) {
-                        const unsigned lo = in && n + 2 * k < P.N ? p[2 * k] : 0u, hi = in && n + 2 * k + 1 < P.N ? p[2 * k + 1] : 0u;
+                        const unsigned lo = n + 2 * k < P.N ? p[2 * k] : 0u, hi = n + 2 * k + 1 < P.N ? p[2 * k + 1] : 0u;
                         st.a[j][k] = lo | (hi << 16);
                     }
                 }
-                const uint8_t* q = P.q + row * P.ldq + c;
+                const uint8_t* q = P.q + r * P.ldq + (cin ? c : 0);
 #pragma unroll
-                for (int k = 0; k < PC / 4; ++k) st.q[j][k] = in && cin ? *reinterpret_cast<const unsigned*>(q + 4 * k) : 0u;
-                st.s[j] = in && cin ? P.scale[row * P.CB + (c >> 5)] : 0u;
+                for (int k = 0; k < PC / 4; ++k) st.q[j][k] = *reinterpret_cast<const unsigned*>(q + 4 * k);
+                st.s[j] = P.scale[r * P.CB + (cin ? c >> 5 : 0)];
+                if (!in) {
+#pragma unroll
+                    for (int k = 0; k < AD; ++k) st.a[j][k] = 0u;
+                }
+                if (!in || !cin) {
+#pragma unroll
+                    for (int k = 0; k < PC / 4; ++k) st.q[j][k] = 0u;
+                    st.s[j] = 0u;
+                }
             }
         }
     }
@@ -432,8 +445,8 @@ extern "C" int y5m_act8_wgrad(const void* dy, int64_t dy_batch_stride, int64_t d
     Y5M_REQUIRE(((uintptr_t)ws & 15) == 0 && ws && ws_bytes >= y5m_act8_wgrad_workspace_bytes(N * S, Cout, C), "workspace too small or not 16-byte aligned");
     // rows of all samples at one distance in whole vector pieces, and a range of them within a buffer resource's 32-bit offsets
     const int64_t pitch = S == 1 && N > 1 ? dy_batch_stride : dy_row_stride;      // (one row per sample: the samples are the rows)
-    bool fast = rows_aligned16(dy, dy_batch_stride, dy_row_stride, N, S, Cout, dtype) && (N == 1 || S == 1 || dy_batch_stride == S * dy_row_stride) &&
-                pitch >= Cout && pitch < (1 << 24);
+    const bool flat = N == 1 || S == 1 || dy_batch_stride == S * dy_row_stride;
+    bool fast = flat && rows_aligned16(dy, dy_batch_stride, dy_row_stride, N, S, Cout, dtype) && pitch >= Cout && pitch < (1 << 24);
     AwParams P = {};
     AwShape s = aw_shape(Cout, C, fast && dtype == Y5M_BF16);
     aw_geometry(P, s, N * S, Cout, C);
@@ -442,7 +455,7 @@ extern "C" int y5m_act8_wgrad(const void* dy, int64_t dy_batch_stride, int64_t d
         s = aw_shape(Cout, C, false);
         aw_geometry(P, s, N * S, Cout, C);
     }
-    P.dy = dy; P.dn = dy_batch_stride; P.dr = fast ? pitch : dy_row_stride; P.S = S;
+    P.dy = dy; P.dn = dy_batch_stride; P.dr = flat ? pitch : dy_row_stride; P.S = flat ? 0 : S;
     P.q = static_cast<const uint8_t*>(q); P.scale = static_cast<const uint8_t*>(scale); P.ldq = ldq;
     P.part = static_cast<float*>(ws);
     P.dbpart = db ? P.part + (size_t)P.ranges * Cout * C : nullptr;

@@ -5,15 +5,19 @@
 //   backward  from x or its 8-bit form:  dt = dz act'(t),  dbeta_c = sum dt,  dgamma_c = sum dt xhat  (over n and rows)
 //             dx = rstd (gamma dt - A - xhat B),  A = sum_group(gamma dt) / K,  B = sum_group(gamma dt xhat) / K
 //
-// All of it is bound by bytes. The statistics of a group must be complete before its first output, so either the values stay on the
-// chip between the two (not here) or they are read twice:
-//   split form: a reduce pass over row chunks (partial sums per channel and chunk, f32), a small launch that joins the chunks in a
-//   fixed order in f64, and an apply pass. No atomics: the result does not depend on the order in which workgroups run.
-// A thread owns 8 channels of a row (16 bytes of bf16) for the whole launch, so gamma / beta / mean / rstd sit in registers and
-// consecutive lanes read consecutive pieces of consecutive rows, whatever D is: groups are cut out when the channel sums are joined,
-// never by the loads (at 96 channels in 32 groups a group is 6 bytes wide).
-// Sums of squares are taken about a pivot per (n, channel), the median of three of its rows: sum (x - p)^2 - (sum (x - p))^2 / S
-// cancels only by how far p lies from the mean, and the median keeps a single outlier row from becoming the pivot.
+// All of it is bound by bytes; the statistics of a group must be complete before its first output. Two forms:
+//   held (gn_held_*): a workgroup loads all rows of a slice of whole groups of one sample into registers, reduces, applies, stores: every
+//     byte is touched once, one launch (the backward's sums over the samples take a second, small one). For small maps, where launches
+//     are what costs;
+//   split: a reduce pass over row chunks, a small launch that joins the chunks in f64, an apply pass that reads the rows again.
+// Neither uses atomics: the result does not depend on the order in which workgroups run. What else was built and measured, at
+// 64 x 160 x 160 x 96 in bf16 with the int8 form (forward + backward): one launch whose workgroups wait for each other's sums (their
+// round trips past the L2s and the registers of the join cost more than the second read: 604 us at best), batches of samples whose
+// rows fit the memory-side cache between the two reads (653 us: the apply pass is bound by its writes), 300 KB slices held at 40 rows
+// a thread (spills: 186 us for the forward at 40 x 40 x 384, split 69).
+// A thread owns 8 channels of a row (16 bytes of bf16), so gamma / beta / mean / rstd sit in registers, and consecutive lanes read
+// consecutive pieces of consecutive rows, whatever D is: groups are cut out when the channel sums are joined, never by the loads (at 96
+// channels in 32 groups a group is 6 bytes wide).
 #include "y5m_act8.h"
 
 #define GN_THREADS 256
@@ -25,17 +29,20 @@ struct GnParams {
     const float *gamma, *beta;     // null: 1, 0
     float *mean, *rstd;            // [N][G]
     uint8_t *q, *scale;            // 8-bit form
-    float* part;                   // [N][chunks][2][C] channel sums of the reduce pass
-    float* nc;                     // backward: [N][2][C] channel sums
-    float* ab;                     // backward: [N][G][2] A, B
+    float* part;                   // split: [N][chunks][C][2] channel sums: mean and M2 of the chunk; backward: sum dt, sum dt xhat
+    float* nc;                     // backward: [N][C][2] channel sums
+    float* ab;                     // backward, split: [N][G][2] A, B
     float *dgamma, *dbeta;
     int64_t N, xn, xr, zn, zr, on, orow;
     int S, C, G, D, ldq, CB, act;
     float eps;
-    int CV, ct, tiles, RP, chunks, rpc;      // pieces per row / per column tile, column tiles, rows side by side, row chunks, rows per chunk
-    unsigned main_blocks;                    // backward apply: blocks beyond these reduce dgamma / dbeta
+    int CV, ct, tiles, RP, chunks, rpc;      // split: pieces per row / per column tile, column tiles, rows side by side, row chunks, rows per chunk
+    int achunks, arpc;                       // the apply pass's chunks
+    unsigned ctm, dm;                        // ceil(2^32 / ct), ceil(2^32 / D): quotients of threads and channels by one multiply
+    int sc, slices;                          // held: channels per slice, slices (ct pieces, RP rows side by side)
 };
 
+// ---- arithmetic -----------------------------------------------------------------------------------------------------------------
 template <int DT> __device__ __forceinline__ float gn_sigmoid(float t) {
     const float a = -t;
     float e;
@@ -50,204 +57,290 @@ template <int DT> __device__ __forceinline__ float gn_sigmoid(float t) {
     }
     return __builtin_amdgcn_rcpf(1.0f + e);
 }
-__device__ __forceinline__ float gn_pivot(float a, float b, float c) {
-    return fmaxf(fminf(a, b), fminf(fmaxf(a, b), c));
-}
 
-// sums over the RP rows that a workgroup holds side by side: v[16] = two sums of 8 channels per thread -> dst[which * C + c]
-__device__ __forceinline__ void gn_join_rows(const float* v, float* red, int lr, int lc, int ct, int RP, bool in, int c0, int C, float* __restrict__ dst) {
-    const int w = ct * 16;
-    if (in) {
-#pragma unroll
-        for (int k = 0; k < 16; ++k) red[lr * w + (k >> 3) * (ct * 8) + lc * 8 + (k & 7)] = v[k];
-    }
-    __syncthreads();
-    for (int j = threadIdx.x; j < w; j += GN_THREADS) {
-        const int which = j / (ct * 8), c = c0 + j - which * (ct * 8);
-        if (c >= C) continue;
-        float a = 0.f;
-        for (int r = 0; r < RP; ++r) a += red[r * w + j];
-        dst[(size_t)which * C + c] = a;
-    }
-}
-
+// ---- places -----------------------------------------------------------------------------------------------------------------------
 struct GnPlace { int64_t n; int lr, lc, piece, c, nv, r0, r1, chunk; bool in; };
-__device__ __forceinline__ GnPlace gn_place(const GnParams& P, unsigned blk) {
+// (exact: numerator * divisor < 2^32; the launcher keeps C below 2^16)
+__device__ __forceinline__ int gn_div(int a, unsigned magic) { return magic ? (int)__umulhi((unsigned)a, magic) : a; }
+static unsigned gn_magic(int d) { return d == 1 ? 0u : (unsigned)(((1ull << 32) + d - 1) / d); }
+// grid: (chunks * tiles, samples folded over y and z). The apply pass takes the samples from the last to the first: what the reduce pass
+// read last is still in the memory-side cache
+template <bool BACK> __device__ __forceinline__ GnPlace gn_place(const GnParams& P, int rpc) {
     GnPlace w;
-    const int tile = (int)(blk % (unsigned)P.tiles);
-    blk /= (unsigned)P.tiles;
-    w.chunk = (int)(blk % (unsigned)P.chunks);
-    w.n = blk / (unsigned)P.chunks;
-    w.lr = (int)threadIdx.x / P.ct;
+    const int tile = P.tiles > 1 ? (int)(blockIdx.x % (unsigned)P.tiles) : 0;
+    w.chunk = P.tiles > 1 ? (int)(blockIdx.x / (unsigned)P.tiles) : (int)blockIdx.x;
+    w.n = (int64_t)blockIdx.z * gridDim.y + blockIdx.y;
+    if (BACK) w.n = P.N - 1 - w.n;                                 // (below 0: beyond the last, as w.n >= N)
+    w.lr = gn_div((int)threadIdx.x, P.ctm);
     w.lc = (int)threadIdx.x - w.lr * P.ct;
     w.piece = tile * P.ct + w.lc;
     w.c = w.piece * 8;
     w.nv = P.C - w.c;
     w.in = w.lr < P.RP && w.piece < P.CV && w.nv > 0;
-    w.r0 = w.chunk * P.rpc;
-    w.r1 = w.r0 + P.rpc < P.S ? w.r0 + P.rpc : P.S;
+    w.r0 = w.chunk * rpc;
+    w.r1 = w.r0 + rpc < P.S ? w.r0 + rpc : P.S;
     return w;
 }
-
-// three rows whose median is a channel's pivot
-template <int DT, bool AL> __device__ __forceinline__ void gn_pivots(const GnParams& P, int64_t n, int c, int nv, float p[8]) {
-    typedef typename RowElem<DT>::T T;
-    const T* b = static_cast<const T*>(P.x) + n * P.xn + c;
-    float u[8], v[8], w[8];
-    load8<DT, AL>(b, nv, u);
-    load8<DT, AL>(b + (int64_t)(P.S / 2) * P.xr, nv, v);
-    load8<DT, AL>(b + (int64_t)(P.S - 1) * P.xr, nv, w);
+// group of each of the thread's 8 channels
+struct GnGroups { int g[8]; };
+__device__ __forceinline__ GnGroups gn_groups(const GnParams& P, int c) {
+    GnGroups k;
+    int g = c < P.C ? gn_div(c, P.dm) : 0, left = (g + 1) * P.D - c;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) p[k] = gn_pivot(u[k], v[k], w[k]);
+    for (int i = 0; i < 8; ++i) {
+        k.g[i] = g < P.G ? g : P.G - 1;
+        if (--left == 0) { ++g; left = P.D; }
+    }
+    return k;
 }
 
-template <int DT, bool AL>
+// sums over the RP rows that a workgroup holds side by side: v[16] = two sums of 8 channels per thread. f(channel, sum, sum) for each
+// channel, one thread per channel
+template <typename F>
+__device__ __forceinline__ void gn_join_rows(const float* v, float* red, const GnPlace& w, int ct, int RP, int C, F f) {
+    const int wd = ct * 8, c0 = (w.piece - w.lc) * 8;
+    float* red2 = red + GN_THREADS * 8;
+    if (w.in) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            red[w.lr * wd + w.lc * 8 + k] = v[k];
+            red2[w.lr * wd + w.lc * 8 + k] = v[8 + k];
+        }
+    }
+    __syncthreads();
+    const int parts = GN_THREADS / wd;
+    if (parts < 2) {
+        for (int j = threadIdx.x; j < wd; j += GN_THREADS) {
+            float a = 0.f, b = 0.f;
+            for (int r = 0; r < RP; ++r) {
+                a += red[r * wd + j];
+                b += red2[r * wd + j];
+            }
+            if (c0 + j < C) f(c0 + j, a, b);
+        }
+        return;
+    }
+    // spare threads take every parts-th row; their sums meet in LDS
+    const int part = (int)threadIdx.x / wd, j = (int)threadIdx.x - part * wd;
+    float a = 0.f, b = 0.f;
+    if (part < parts) {
+        int r = part;
+        for (; r + 3 * parts < RP; r += 4 * parts) {
+            float u[4], v4[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) { u[k] = red[(r + k * parts) * wd + j]; v4[k] = red2[(r + k * parts) * wd + j]; }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) { a += u[k]; b += v4[k]; }
+        }
+        for (; r < RP; r += parts) {
+            a += red[r * wd + j];
+            b += red2[r * wd + j];
+        }
+    }
+    __syncthreads();
+    if (part < parts) {
+        red[threadIdx.x] = a;
+        red2[threadIdx.x] = b;
+    }
+    __syncthreads();
+    if (part == 0 && c0 + j < C) {
+        for (int k = 1; k < parts; ++k) {
+            a += red[k * wd + j];
+            b += red2[k * wd + j];
+        }
+        f(c0 + j, a, b);
+    }
+}
+__device__ __forceinline__ float* gn_part(const GnParams& P, const GnPlace& w) { return P.part + ((size_t)w.n * P.chunks + w.chunk) * 2 * P.C; }
+
+// ---- forward, split ---------------------------------------------------------------------------------------------------------------
+// Squares are summed about the chunk's first row: a chunk's mean and M2 = sum (x - p)^2 - (sum (x - p))^2 / R then cancel by at most a
+// factor R (a few hundred), even if that row is an outlier; chunks are joined by the pairwise formula.
+template <int DT, int AL>
 __global__ __launch_bounds__(GN_THREADS) void gn_stats_kernel(const GnParams P) {
     typedef typename RowElem<DT>::T T;
     __shared__ float red[GN_THREADS * 16];
-    const GnPlace w = gn_place(P, blockIdx.x);
-    float a[16];
+    const GnPlace w = gn_place<false>(P, P.rpc);
+    if (w.n >= P.N) return;
+    float a[16], pv[8];
 #pragma unroll
     for (int k = 0; k < 16; ++k) a[k] = 0.f;
+    const T* b = static_cast<const T*>(P.x) + w.n * P.xn + w.c;
     if (w.in) {
-        float p[8];
-        gn_pivots<DT, AL>(P, w.n, w.c, w.nv, p);
-        const T* b = static_cast<const T*>(P.x) + w.n * P.xn + w.c;
+        load8<DT, AL>(b + (int64_t)w.r0 * P.xr, w.nv, pv);
         auto add = [&](const Raw8<DT>& raw) __attribute__((always_inline)) {
             float v[8];
             unpack8<DT>(raw, v);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const float d = v[k] - p[k];
+                const float d = v[k] - pv[k];
                 a[k] += d;
                 a[8 + k] = fmaf(d, d, a[8 + k]);
             }
         };
+        constexpr int U = 4;                                       // rows in flight (8: five waves per SIMD instead of eight, no faster)
+        const int64_t step = (int64_t)P.RP * P.xr;
         int r = w.r0 + w.lr;
-        for (; r + 3 * P.RP < w.r1; r += 4 * P.RP) {
-            Raw8<DT> raw[4];
+        const T* p = b + (int64_t)r * P.xr;
+        for (; r + (U - 1) * P.RP < w.r1; r += U * P.RP) {
+            Raw8<DT> raw[U];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) raw[u] = load_raw8<DT, AL>(b + (int64_t)(r + u * P.RP) * P.xr, w.nv);
+            for (int u = 0; u < U; ++u) {
+                raw[u] = load_raw8<DT, AL>(p, w.nv);
+                p += step;
+            }
 #pragma unroll
-            for (int u = 0; u < 4; ++u) add(raw[u]);
+            for (int u = 0; u < U; ++u) add(raw[u]);
         }
-        for (; r < w.r1; r += P.RP) add(load_raw8<DT, AL>(b + (int64_t)r * P.xr, w.nv));
+        for (; r < w.r1; r += P.RP) {
+            add(load_raw8<DT, AL>(p, w.nv));
+            p += step;
+        }
     }
-    gn_join_rows(a, red, w.lr, w.lc, P.ct, P.RP, w.in, (w.piece - w.lc) * 8, P.C, P.part + ((size_t)w.n * P.chunks + w.chunk) * 2 * P.C);
+    // channel sums about the first row -> the chunk's mean and M2
+    float* dst = gn_part(P, w);
+    const float R = (float)(w.r1 - w.r0);
+    const T* first = static_cast<const T*>(P.x) + w.n * P.xn + (int64_t)w.r0 * P.xr;
+    gn_join_rows(a, red, w, P.ct, P.RP, P.C, [&](int c, float s1, float s2) __attribute__((always_inline)) {
+        float pv;
+        if constexpr (DT == Y5M_F32) pv = first[c];
+        else if constexpr (DT == Y5M_BF16) pv = bf16_to_f32(first[c]);
+        else pv = f16_to_f32(first[c]);
+        *reinterpret_cast<float2*>(dst + 2 * c) = make_float2(pv + s1 / R, s2 - s1 * s1 / R);
+    });
 }
 
-// one wave per (n, group); lane = (chunk slot, channel of the group)
-__device__ __forceinline__ double gn_shfl_xor(double v, int o) {
-    const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    const unsigned lo = (unsigned)__shfl_xor((int)(unsigned)u, o, 64), hi = (unsigned)__shfl_xor((int)(unsigned)(u >> 32), o, 64);
-    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-}
 __device__ __forceinline__ double gn_wave_sum(double v) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += gn_shfl_xor(v, o);
+    for (int o = 32; o > 0; o >>= 1) {
+        const uint64_t u = __builtin_bit_cast(uint64_t, v);
+        const unsigned lo = (unsigned)__shfl_xor((int)(unsigned)u, o, 64), hi = (unsigned)__shfl_xor((int)(unsigned)(u >> 32), o, 64);
+        v += __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+    }
     return v;
 }
-struct GnSlots { int p2, d0, slot, slots; };
-__device__ __forceinline__ GnSlots gn_slots(int D, int lane) {
-    GnSlots s;
-    s.p2 = 1;
-    while (s.p2 < D && s.p2 < 64) s.p2 <<= 1;
-    s.slots = 64 / s.p2;
-    s.slot = lane / s.p2;
-    s.d0 = lane - s.slot * s.p2;
-    return s;
-}
-// sums of one channel over the row chunks, joined over the slots: every lane of the channel gets both
-__device__ __forceinline__ void gn_channel_sums(const GnParams& P, int64_t n, int c, bool in, const GnSlots& s, double& a, double& b) {
-    a = b = 0.0;
-    if (in)
-        for (int ch = s.slot; ch < P.chunks; ch += s.slots) {
-            const float* p = P.part + ((size_t)n * P.chunks + ch) * 2 * P.C + c;
-            a += (double)p[0];
-            b += (double)p[P.C];
-        }
-    for (int o = 32; o >= s.p2; o >>= 1) {
-        a += gn_shfl_xor(a, o);
-        b += gn_shfl_xor(b, o);
+// a workgroup's sum of NV doubles per thread, in a fixed order; every thread gets it
+template <int NV> __device__ __forceinline__ void gn_block_sum(double* v, double* red) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) v[i] = gn_wave_sum(v[i]);
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) red[i * 4 + (threadIdx.x >> 6)] = v[i];
     }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NV; ++i) v[i] = (red[i * 4] + red[i * 4 + 1]) + (red[i * 4 + 2] + red[i * 4 + 3]);
+    __syncthreads();
+}
+// One workgroup per (sample, group): its chunks x D channels are walked over in pieces of w = min(D, 256) channels, 256 / w chunks side
+// by side. (Latency is all there is: four loads in flight per thread, 4 us where one wave per group took 7.)
+struct GnWalk { int w, slots, slot, d; };
+__device__ __forceinline__ GnWalk gn_walk(int D) {
+    GnWalk k;
+    k.w = D < GN_THREADS ? D : GN_THREADS;
+    k.slots = GN_THREADS / k.w;
+    k.slot = (int)threadIdx.x / k.w;
+    k.d = (int)threadIdx.x - k.slot * k.w;
+    return k;
 }
 
-template <int DT>
 __global__ __launch_bounds__(GN_THREADS) void gn_stats_join_kernel(const GnParams P) {
-    typedef typename RowElem<DT>::T T;
-    const int lane = threadIdx.x & 63;
-    const int64_t ng = (int64_t)blockIdx.x * (GN_THREADS / 64) + (threadIdx.x >> 6);
-    if (ng >= P.N * P.G) return;                                   // (whole waves)
-    const int64_t n = ng / P.G;
-    const int g = (int)(ng - n * P.G);
-    const GnSlots s = gn_slots(P.D, lane);
-    const double S = (double)P.S;
-    double m1 = 0.0, m2 = 0.0, mm = 0.0, ref = 0.0;                // sum of channel means (about ref), of M2, of squared means (about ref)
-    for (int db = 0; db < P.D; db += s.p2) {
-        const int d = db + s.d0, c = g * P.D + d;
-        const bool in = d < P.D;
-        double a, b;
-        gn_channel_sums(P, n, c, in, s, a, b);
-        double cm = 0.0;
-        if (in) {
-            float u, v, w;
-            const T* x = static_cast<const T*>(P.x) + n * P.xn + c;
-            if constexpr (DT == Y5M_F32) { u = x[0]; v = x[(int64_t)(P.S / 2) * P.xr]; w = x[(int64_t)(P.S - 1) * P.xr]; }
-            else if constexpr (DT == Y5M_BF16) { u = bf16_to_f32(x[0]); v = bf16_to_f32(x[(int64_t)(P.S / 2) * P.xr]); w = bf16_to_f32(x[(int64_t)(P.S - 1) * P.xr]); }
-            else { u = f16_to_f32(x[0]); v = f16_to_f32(x[(int64_t)(P.S / 2) * P.xr]); w = f16_to_f32(x[(int64_t)(P.S - 1) * P.xr]); }
-            cm = (double)gn_pivot(u, v, w) + a / S;
+    __shared__ double red[12];
+    const int64_t b = blockIdx.x / (unsigned)P.G;
+    const int g = (int)(blockIdx.x - b * P.G);
+    const float* part = P.part + (size_t)b * P.chunks * 2 * P.C + 2 * g * P.D;
+    const GnWalk k = gn_walk(P.D);
+    const double ref = (double)part[0];
+    double v[3] = {0.0, 0.0, 0.0};                                 // sum R (m - ref), sum R (m - ref)^2, sum M2
+    if (k.slot < k.slots)
+        for (int d = k.d; d < P.D; d += GN_THREADS) {
+            auto add = [&](const float2& m, int ch) __attribute__((always_inline)) {
+                const double R = (double)(ch + 1 < P.chunks ? P.rpc : P.S - ch * P.rpc), e = (double)m.x - ref;
+                v[0] += R * e;
+                v[1] += R * e * e;
+                v[2] += (double)m.y;
+            };
+            int ch = k.slot;
+            for (; ch + 3 * k.slots < P.chunks; ch += 4 * k.slots) {
+                float2 m[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) m[u] = *reinterpret_cast<const float2*>(part + (size_t)(ch + u * k.slots) * 2 * P.C + 2 * d);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) add(m[u], ch + u * k.slots);
+            }
+            for (; ch < P.chunks; ch += k.slots) add(*reinterpret_cast<const float2*>(part + (size_t)ch * 2 * P.C + 2 * d), ch);
         }
-        if (db == 0) {                                             // about the first channel's mean: its lane is lane 0
-            const uint64_t u = __builtin_bit_cast(uint64_t, cm);
-            const unsigned lo = (unsigned)__shfl((int)(unsigned)u, 0, 64), hi = (unsigned)__shfl((int)(unsigned)(u >> 32), 0, 64);
-            ref = __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-        }
-        if (in && s.slot == 0) {
-            m1 += cm - ref;
-            mm += (cm - ref) * (cm - ref);
-            m2 += b - a * a / S;
-        }
-    }
-    m1 = gn_wave_sum(m1);
-    m2 = gn_wave_sum(m2);
-    mm = gn_wave_sum(mm);
-    const double D = (double)P.D;
-    double var = m2 / (S * D) + mm / D - (m1 / D) * (m1 / D);
-    if (!(var > 0.0) && var == var) var = 0.0;                     // (a NaN stays)
-    if (lane == 0) {
-        P.mean[ng] = (float)(ref + m1 / D);
+    gn_block_sum<3>(v, red);
+    if (threadIdx.x == 0) {
+        const double K = (double)P.S * (double)P.D, off = v[0] / K;
+        double var = v[2] / K + v[1] / K - off * off;
+        if (!(var > 0.0) && var == var) var = 0.0;                 // (a NaN stays)
+        const int64_t ng = b * P.G + g;
+        P.mean[ng] = (float)(ref + off);
         P.rstd[ng] = (float)(1.0 / sqrt(var + (double)P.eps));
     }
 }
 
-struct GnCoef { float mean[8], rstd[8], gamma[8], beta[8]; };
-__device__ __forceinline__ void gn_coef(const GnParams& P, const GnPlace& w, GnCoef& k) {
+// coefficients of a thread's 8 channels
+// 8 values of a per-channel parameter (absent: `none`)
+__device__ __forceinline__ void gn_param8(const float* __restrict__ p, int c, int nv, float none, float* v) {
+    if (p && nv >= 8) {
+        __builtin_memcpy(v, p + c, 32);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int c = w.c + i < P.C ? w.c + i : P.C - 1, g = c / P.D;
-        k.mean[i] = P.mean[w.n * P.G + g];
-        k.rstd[i] = P.rstd[w.n * P.G + g];
-        k.gamma[i] = P.gamma ? P.gamma[c] : 1.0f;
-        k.beta[i] = P.beta ? P.beta[c] : 0.0f;
+        for (int i = 0; i < 8; ++i) v[i] = p ? p[c + (i < nv ? i : nv - 1)] : none;
     }
 }
+struct GnCoef { float mean[8], rstd[8], gamma[8], beta[8]; };
+__device__ __forceinline__ void gn_stat8(const GnParams& P, const GnPlace& w, const GnGroups& gr, GnCoef& k) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        k.mean[i] = P.mean[w.n * P.G + gr.g[i]];
+        k.rstd[i] = P.rstd[w.n * P.G + gr.g[i]];
+    }
+}
+__device__ __forceinline__ void gn_coef(const GnParams& P, const GnPlace& w, const GnGroups& gr, GnCoef& k) {
+    gn_stat8(P, w, gr, k);
+    const int c = w.in ? w.c : 0, nv = w.in ? w.nv : P.C;
+    gn_param8(P.gamma, c, nv, 1.0f, k.gamma);
+    gn_param8(P.beta, c, nv, 0.0f, k.beta);
+}
 
-template <int DT, bool AL, int FMT>
+// t = gamma xhat + beta. f32: (x - mean) first, exact where x is near the mean. 16 bits: one fma, x a + b -- its rounding of |mean| a
+// is 2^-24 where x's own type already cost 2^-9 or 2^-12 of the same
+template <int DT> struct GnAffine {
+    float a[8], b[8], m[DT == Y5M_F32 ? 8 : 1];
+    __device__ __forceinline__ void set(const GnCoef& k) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            a[i] = k.rstd[i] * k.gamma[i];
+            if constexpr (DT == Y5M_F32) { m[i] = k.mean[i]; b[i] = k.beta[i]; }
+            else b[i] = fmaf(-k.mean[i], a[i], k.beta[i]);
+        }
+    }
+    __device__ __forceinline__ float operator()(float v, int i) const {
+        if constexpr (DT == Y5M_F32) return fmaf(v - m[i], a[i], b[i]);
+        else return fmaf(v, a[i], b[i]);
+    }
+};
+
+template <int DT, int AL, int FMT>
 __global__ __launch_bounds__(GN_THREADS) void gn_apply_kernel(const GnParams P) {
     typedef typename RowElem<DT>::T T;
-    const GnPlace w = gn_place(P, blockIdx.x);
-    GnCoef k;
-    if (w.in) {
-        gn_coef(P, w, k);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) k.rstd[i] *= k.gamma[i];
+    const GnPlace w = gn_place<true>(P, P.arpc);
+    if (w.n < 0) return;
+    const GnGroups gr = gn_groups(P, w.c);
+    GnAffine<DT> af;
+    {
+        GnCoef k;
+        gn_coef(P, w, gr, k);
+        af.set(k);
     }
     const bool silu = P.act == Y5M_ACT_SILU;
-    const T* b = static_cast<const T*>(P.x) + w.n * P.xn + w.c;
+    const T* b = static_cast<const T*>(P.x) + w.n * P.xn + (w.in ? w.c : 0);
     T* o = static_cast<T*>(P.out) + w.n * P.on + w.c;
     // Every lane runs the same trips (the four lanes of a block must meet in the encoder): rows and pieces beyond the end are read
     // from the last row / the first piece instead, which is in bounds, and not stored.
-    const T* bl = w.in ? b : static_cast<const T*>(P.x) + w.n * P.xn;
     const int nvl = w.in ? w.nv : P.C;
     auto finish = [&](const Raw8<DT>& raw, int r) __attribute__((always_inline)) {
         const bool live = w.in && r < w.r1;
@@ -267,33 +360,35 @@ __global__ __launch_bounds__(GN_THREADS) void gn_apply_kernel(const GnParams P) 
         if (live) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float t = fmaf(v[i] - k.mean[i], k.rstd[i], k.beta[i]);
+                const float t = af(v[i], i);
                 z[i] = silu ? t * gn_sigmoid<DT>(t) : t;
             }
             store8<DT, AL>(o + (int64_t)r * P.orow, w.nv, z);
         }
     };
     const int lr = w.lr < P.RP ? w.lr : 0;
+    const int64_t step = (int64_t)P.RP * P.xr;
+    const T *p = b + (int64_t)(w.r0 + lr) * P.xr, *end = b + (int64_t)(w.r1 - 1) * P.xr;
     for (int rb = w.r0; rb < w.r1; rb += 4 * P.RP) {
         Raw8<DT> raw[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            const int r = rb + lr + u * P.RP;
-            raw[u] = load_raw8<DT, AL>(bl + (int64_t)(r < w.r1 ? r : w.r1 - 1) * P.xr, nvl);
+            raw[u] = load_raw8<DT, AL>(rb + lr + u * P.RP < w.r1 ? p : end, nvl);
+            p += step;
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u) finish(raw[u], rb + lr + u * P.RP);
     }
 }
 
-// ---- backward -----------------------------------------------------------------------------------------------------------------
+// ---- backward, split ---------------------------------------------------------------------------------------------------------------
 // the kept input of one row piece: x itself or its 8-bit form
 template <int DT, int FMT> struct GnKept {
     Raw8<DT> raw;
 };
 template <int DT> struct GnKept<DT, Y5M_KEEP_E4M3> { act8_u32x2 q; unsigned s; };
 template <int DT> struct GnKept<DT, Y5M_KEEP_INT8> { act8_u32x2 q; unsigned s; };
-template <int DT, bool AL, int FMT>
+template <int DT, int AL, int FMT>
 __device__ __forceinline__ GnKept<DT, FMT> gn_kept(const GnParams& P, const GnPlace& w, int r) {
     typedef typename RowElem<DT>::T T;
     GnKept<DT, FMT> k;
@@ -310,186 +405,672 @@ template <int DT, int FMT> __device__ __forceinline__ void gn_kept_values(const 
     if constexpr (FMT == Y5M_KEEP_NONE) unpack8<DT>(k.raw, v);
     else act8_decode8<FMT>(k.q, act8_scale(k.s), v);
 }
+// a thread's rows r, r + RP, ...: what was kept and the incoming gradient, by pointers that step
+template <int DT, int AL, int FMT> struct GnCursor {
+    typedef typename RowElem<DT>::T T;
+    const T *x, *d;
+    const uint8_t *q, *s;
+    int64_t xs, ds, qs, ss;
+    int nv;
+    __device__ __forceinline__ GnCursor(const GnParams& P, const GnPlace& w, int r, const T* dz) {
+        nv = w.nv;
+        d = dz + (int64_t)r * P.zr;
+        ds = (int64_t)P.RP * P.zr;
+        if constexpr (FMT == Y5M_KEEP_NONE) {
+            x = static_cast<const T*>(P.x) + w.n * P.xn + (int64_t)r * P.xr + w.c;
+            xs = (int64_t)P.RP * P.xr;
+        } else {
+            const int64_t row = w.n * P.S + r;
+            q = P.q + row * P.ldq + w.c;
+            s = P.scale + row * P.CB + (w.piece >> 2);
+            qs = (int64_t)P.RP * P.ldq;
+            ss = (int64_t)P.RP * P.CB;
+        }
+    }
+    __device__ __forceinline__ void next(GnKept<DT, FMT>& k, Raw8<DT>& g) {
+        if constexpr (FMT == Y5M_KEEP_NONE) {
+            k.raw = load_raw8<DT, AL>(x, nv);
+            x += xs;
+        } else {
+            k.q = *reinterpret_cast<const act8_u32x2*>(q);
+            k.s = *s;
+            q += qs;
+            s += ss;
+        }
+        g = load_raw8<DT, AL>(d, nv);
+        d += ds;
+    }
+};
 template <int DT> __device__ __forceinline__ float gn_act_grad(bool silu, float t) {
     const float s = gn_sigmoid<DT>(t);
     return silu ? s * fmaf(t, 1.0f - s, 1.0f) : 1.0f;
 }
-
-template <int DT, bool AL, int FMT>
-__global__ __launch_bounds__(GN_THREADS) void gn_bwd_reduce_kernel(const GnParams P) {
-    typedef typename RowElem<DT>::T T;
-    __shared__ float red[GN_THREADS * 16];
-    const GnPlace w = gn_place(P, blockIdx.x);
-    float a[16];
+// xhat = (x - mean) rstd, for 16-bit types as one fma (GnAffine says why)
+template <int DT> __device__ __forceinline__ float gn_xhat(float v, const GnCoef& k, int i) {
+    if constexpr (DT == Y5M_F32) return (v - k.mean[i]) * k.rstd[i];
+    else return fmaf(v, k.rstd[i], k.mean[i]);
+}
+template <int DT> __device__ __forceinline__ void gn_coef_xhat(GnCoef& k) {
+    if constexpr (DT != Y5M_F32) {
 #pragma unroll
-    for (int k = 0; k < 16; ++k) a[k] = 0.f;
-    if (w.in) {
+        for (int i = 0; i < 8; ++i) k.mean[i] = -k.mean[i] * k.rstd[i];
+    }
+}
+
+// dt = dz act'(t) of one piece. f32: through xhat, which comes back in v. 16 bits: v stays the kept value and u = -t log2(e) is one
+// fma of it (GnAffine says why that is enough): act'(t) = s (1 + t (1 - s)), s = 1 / (1 + 2^u), t (1 - s) = u (ln2 s - ln2)
+template <int DT> struct GnGrad {
+    float a[8], b[8], m[DT == Y5M_F32 ? 8 : 1], r[DT == Y5M_F32 ? 8 : 1];
+    __device__ __forceinline__ void set(const GnCoef& k) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if constexpr (DT == Y5M_F32) {
+                a[i] = k.gamma[i];
+                b[i] = k.beta[i];
+                m[i] = k.mean[i];
+                r[i] = k.rstd[i];
+            } else {
+                a[i] = k.gamma[i] * k.rstd[i];
+                b[i] = -1.44269502f * fmaf(-k.mean[i], a[i], k.beta[i]);
+                a[i] *= -1.44269502f;
+            }
+        }
+    }
+    template <bool SILU> __device__ __forceinline__ void operator()(float* v, float* g) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if constexpr (DT == Y5M_F32) {
+                v[i] = (v[i] - m[i]) * r[i];
+                if constexpr (SILU) g[i] *= gn_act_grad<DT>(true, fmaf(v[i], a[i], b[i]));
+            } else if constexpr (SILU) {
+                const float u = fmaf(v[i], a[i], b[i]);
+                const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(u));
+                // (2^u past the largest f32: s = 0 and u may be large, never infinite for finite x)
+                g[i] *= s * fmaf(u, fmaf(s, 0.693147182f, -0.693147182f), 1.0f);
+            }
+        }
+    }
+};
+
+template <int DT, int AL, int FMT, bool SILU>
+__device__ __forceinline__ void gn_bwd_sums(const GnParams& P, const GnPlace& w, const GnGroups& gr, float* a) {
+    typedef typename RowElem<DT>::T T;
+    GnGrad<DT> grad;
+    {
         GnCoef k;
-        gn_coef(P, w, k);
-        const bool silu = P.act == Y5M_ACT_SILU;
-        const T* d = static_cast<const T*>(P.dz) + w.n * P.zn + w.c;
-        auto add = [&](const GnKept<DT, FMT>& kept, const Raw8<DT>& graw) __attribute__((always_inline)) {
-            float v[8], g[8];
-            gn_kept_values<DT, FMT>(kept, v);
-            unpack8<DT>(graw, g);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float xh = (v[i] - k.mean[i]) * k.rstd[i];
-                const float dt = g[i] * gn_act_grad<DT>(silu, fmaf(xh, k.gamma[i], k.beta[i]));
-                a[i] += dt;
-                a[8 + i] = fmaf(dt, xh, a[8 + i]);
-            }
-        };
-        int r = w.r0 + w.lr;
-        for (; r + P.RP < w.r1; r += 2 * P.RP) {
-            GnKept<DT, FMT> kept[2];
-            Raw8<DT> graw[2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                kept[u] = gn_kept<DT, AL, FMT>(P, w, r + u * P.RP);
-                graw[u] = load_raw8<DT, AL>(d + (int64_t)(r + u * P.RP) * P.zr, w.nv);
-            }
-#pragma unroll
-            for (int u = 0; u < 2; ++u) add(kept[u], graw[u]);
-        }
-        for (; r < w.r1; r += P.RP) add(gn_kept<DT, AL, FMT>(P, w, r), load_raw8<DT, AL>(d + (int64_t)r * P.zr, w.nv));
+        gn_coef(P, w, gr, k);
+        grad.set(k);
     }
-    gn_join_rows(a, red, w.lr, w.lc, P.ct, P.RP, w.in, (w.piece - w.lc) * 8, P.C, P.part + ((size_t)w.n * P.chunks + w.chunk) * 2 * P.C);
-}
-
-__global__ __launch_bounds__(GN_THREADS) void gn_bwd_join_kernel(const GnParams P) {
-    const int lane = threadIdx.x & 63;
-    const int64_t ng = (int64_t)blockIdx.x * (GN_THREADS / 64) + (threadIdx.x >> 6);
-    if (ng >= P.N * P.G) return;
-    const int64_t n = ng / P.G;
-    const int g = (int)(ng - n * P.G);
-    const GnSlots s = gn_slots(P.D, lane);
-    double A = 0.0, B = 0.0;
-    for (int db = 0; db < P.D; db += s.p2) {
-        const int d = db + s.d0, c = g * P.D + d;
-        const bool in = d < P.D;
-        double a, b;
-        gn_channel_sums(P, n, c, in, s, a, b);
-        if (in && s.slot == 0) {
-            const double ga = P.gamma ? (double)P.gamma[c] : 1.0;
-            A += ga * a;
-            B += ga * b;
-            P.nc[((size_t)n * 2 + 0) * P.C + c] = (float)a;
-            P.nc[((size_t)n * 2 + 1) * P.C + c] = (float)b;
-        }
-    }
-    A = gn_wave_sum(A);
-    B = gn_wave_sum(B);
-    if (lane == 0) {
-        const double K = (double)P.S * (double)P.D;
-        P.ab[ng * 2 + 0] = (float)(A / K);
-        P.ab[ng * 2 + 1] = (float)(B / K);
-    }
-}
-
-template <int DT, bool AL, int FMT>
-__global__ __launch_bounds__(GN_THREADS) void gn_bwd_apply_kernel(const GnParams P) {
-    typedef typename RowElem<DT>::T T;
-    if (blockIdx.x >= P.main_blocks) {
-        // dbeta / dgamma: 16 channels x 16 sample slots per block, joined in a fixed order in f64
-        __shared__ double acc[2][16][17];
-        const int c = (int)(blockIdx.x - P.main_blocks) * 16 + (threadIdx.x & 15), slot = threadIdx.x >> 4;
-        double a = 0.0, b = 0.0;
-        if (c < P.C)
-            for (int64_t n = slot; n < P.N; n += 16) {
-                a += (double)P.nc[((size_t)n * 2 + 0) * P.C + c];
-                b += (double)P.nc[((size_t)n * 2 + 1) * P.C + c];
-            }
-        acc[0][slot][threadIdx.x & 15] = a;
-        acc[1][slot][threadIdx.x & 15] = b;
-        __syncthreads();
-        if (slot < 2 && c < P.C) {
-            double t = 0.0;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) t += acc[slot][i][threadIdx.x & 15];
-            float* dst = slot == 0 ? P.dbeta : P.dgamma;
-            if (dst) dst[c] = (float)t;
-        }
-        return;
-    }
-    const GnPlace w = gn_place(P, blockIdx.x);
-    if (!w.in) return;
-    GnCoef k;
-    gn_coef(P, w, k);
-    float ra[8], rb[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int c = w.c + i < P.C ? w.c + i : P.C - 1, g = c / P.D;
-        ra[i] = P.ab[(w.n * P.G + g) * 2 + 0];
-        rb[i] = P.ab[(w.n * P.G + g) * 2 + 1];
-    }
-    const bool silu = P.act == Y5M_ACT_SILU;
-    const T* d = static_cast<const T*>(P.dz) + w.n * P.zn + w.c;
-    T* o = static_cast<T*>(P.out) + w.n * P.on + w.c;
-    auto finish = [&](const GnKept<DT, FMT>& kept, const Raw8<DT>& graw, int r) __attribute__((always_inline)) {
+    auto add = [&](const GnKept<DT, FMT>& kept, const Raw8<DT>& graw) __attribute__((always_inline)) {
         float v[8], g[8];
         gn_kept_values<DT, FMT>(kept, v);
         unpack8<DT>(graw, g);
+        grad.template operator()<SILU>(v, g);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float xh = (v[i] - k.mean[i]) * k.rstd[i];
-            const float dt = g[i] * gn_act_grad<DT>(silu, fmaf(xh, k.gamma[i], k.beta[i]));
-            g[i] = k.rstd[i] * (fmaf(k.gamma[i], dt, -ra[i]) - xh * rb[i]);
+            a[i] += g[i];
+            a[8 + i] = fmaf(g[i], v[i], a[8 + i]);
         }
-        store8<DT, AL>(o + (int64_t)r * P.orow, w.nv, g);
     };
     int r = w.r0 + w.lr;
+    GnCursor<DT, AL, FMT> at(P, w, r, static_cast<const T*>(P.dz) + w.n * P.zn + w.c);
+    // (two rows in flight: four cost a quarter of the waves and 30 % of the time)
     for (; r + P.RP < w.r1; r += 2 * P.RP) {
         GnKept<DT, FMT> kept[2];
         Raw8<DT> graw[2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            kept[u] = gn_kept<DT, AL, FMT>(P, w, r + u * P.RP);
-            graw[u] = load_raw8<DT, AL>(d + (int64_t)(r + u * P.RP) * P.zr, w.nv);
-        }
+        for (int u = 0; u < 2; ++u) at.next(kept[u], graw[u]);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) finish(kept[u], graw[u], r + u * P.RP);
+        for (int u = 0; u < 2; ++u) add(kept[u], graw[u]);
     }
-    for (; r < w.r1; r += P.RP) finish(gn_kept<DT, AL, FMT>(P, w, r), load_raw8<DT, AL>(d + (int64_t)r * P.zr, w.nv), r);
+    for (; r < w.r1; r += P.RP) {
+        GnKept<DT, FMT> kept;
+        Raw8<DT> graw;
+        at.next(kept, graw);
+        add(kept, graw);
+    }
+    if constexpr (DT != Y5M_F32) {
+        // sum dt x -> sum dt xhat
+        GnCoef k;
+        gn_stat8(P, w, gr, k);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a[8 + i] = k.rstd[i] * fmaf(-k.mean[i], a[i], a[8 + i]);
+    }
+}
+
+template <int DT, int AL, int FMT>
+__global__ __launch_bounds__(GN_THREADS) void gn_bwd_reduce_kernel(const GnParams P) {
+    __shared__ float red[GN_THREADS * 16];
+    const GnPlace w = gn_place<false>(P, P.rpc);
+    if (w.n >= P.N) return;
+    float a[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) a[k] = 0.f;
+    if (w.in) {
+        const GnGroups gr = gn_groups(P, w.c);
+        if (P.act == Y5M_ACT_SILU) gn_bwd_sums<DT, AL, FMT, true>(P, w, gr, a);
+        else gn_bwd_sums<DT, AL, FMT, false>(P, w, gr, a);
+    }
+    float* dst = gn_part(P, w);
+    gn_join_rows(a, red, w, P.ct, P.RP, P.C, [&](int c, float s0, float s1) __attribute__((always_inline)) { *reinterpret_cast<float2*>(dst + 2 * c) = make_float2(s0, s1); });
+}
+
+// channel sums of a sample and A, B of its groups, one workgroup per (sample, group)
+__global__ __launch_bounds__(GN_THREADS) void gn_bwd_join_kernel(const GnParams P) {
+    __shared__ double red[2 * GN_THREADS];
+    const int64_t b = blockIdx.x / (unsigned)P.G, n = b;
+    const int g = (int)(blockIdx.x - b * P.G);
+    const float* part = P.part + (size_t)b * P.chunks * 2 * P.C + 2 * g * P.D;
+    const GnWalk k = gn_walk(P.D);
+    double v[2] = {0.0, 0.0};
+    for (int d0 = 0; d0 < P.D; d0 += GN_THREADS) {                 // (uniform: every thread meets at the barriers)
+        const int d = d0 + k.d;
+        const bool in = k.slot < k.slots && d < P.D;
+        double s0 = 0.0, s1 = 0.0;
+        if (in) {
+            int ch = k.slot;
+            for (; ch + 3 * k.slots < P.chunks; ch += 4 * k.slots) {
+                float2 m[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) m[u] = *reinterpret_cast<const float2*>(part + (size_t)(ch + u * k.slots) * 2 * P.C + 2 * d);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) { s0 += (double)m[u].x; s1 += (double)m[u].y; }
+            }
+            for (; ch < P.chunks; ch += k.slots) {
+                const float2 m = *reinterpret_cast<const float2*>(part + (size_t)ch * 2 * P.C + 2 * d);
+                s0 += (double)m.x;
+                s1 += (double)m.y;
+            }
+        }
+        red[threadIdx.x] = s0;
+        red[GN_THREADS + threadIdx.x] = s1;
+        __syncthreads();
+        if (in && k.slot == 0) {
+            for (int sl = 1; sl < k.slots; ++sl) {
+                s0 += red[sl * k.w + k.d];
+                s1 += red[GN_THREADS + sl * k.w + k.d];
+            }
+            const int c = g * P.D + d;
+            *reinterpret_cast<float2*>(P.nc + ((size_t)n * P.C + c) * 2) = make_float2((float)s0, (float)s1);
+            const double ga = P.gamma ? (double)P.gamma[c] : 1.0;
+            v[0] += ga * s0;
+            v[1] += ga * s1;
+        }
+        __syncthreads();
+    }
+    gn_block_sum<2>(v, red);
+    if (threadIdx.x == 0) {
+        const double K = (double)P.S * (double)P.D;
+        float* ab = P.ab + (n * P.G + g) * 2;
+        ab[0] = (float)(v[0] / K);
+        ab[1] = (float)(v[1] / K);
+    }
+}
+
+// dbeta / dgamma: the samples' channel sums, 16 channels x 16 sample slots per workgroup, joined in a fixed order in f64
+__global__ __launch_bounds__(GN_THREADS) void gn_param_grad_kernel(const GnParams P) {
+    __shared__ double acc[2][16][17];
+    const int cl = threadIdx.x & 15, c = (int)blockIdx.x * 16 + cl, slot = threadIdx.x >> 4;
+    double a = 0.0, b = 0.0;
+    if (c < P.C) {
+        const float* p = P.nc + ((size_t)slot * P.C + c) * 2;
+        const size_t st = (size_t)P.C * 32;
+        int64_t n = slot;
+        for (; n + 48 < P.N; n += 64, p += 4 * st) {
+            float2 m[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) m[u] = *reinterpret_cast<const float2*>(p + u * st);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) { a += (double)m[u].x; b += (double)m[u].y; }
+        }
+        for (; n < P.N; n += 16, p += st) {
+            const float2 m = *reinterpret_cast<const float2*>(p);
+            a += (double)m.x;
+            b += (double)m.y;
+        }
+    }
+    acc[0][slot][cl] = a;
+    acc[1][slot][cl] = b;
+    __syncthreads();
+    if (slot < 2 && c < P.C) {
+        double t = 0.0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) t += acc[slot][i][cl];
+        float* dst = slot == 0 ? P.dbeta : P.dgamma;
+        if (dst) dst[c] = (float)t;
+    }
+}
+
+template <int DT, int AL, int FMT, bool SILU>
+__device__ __forceinline__ void gn_bwd_rows(const GnParams& P, const GnPlace& w) {
+    typedef typename RowElem<DT>::T T;
+    // dx = r gamma dt - r A - r B xhat = c1 dt + (c2 v + c3), v = xhat in f32, the kept value in 16 bits
+    GnGrad<DT> grad;
+    float c1[8], c2[8], c3[8];
+    {
+        const GnGroups gr = gn_groups(P, w.c);
+        GnCoef k;
+        gn_coef(P, w, gr, k);
+        grad.set(k);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float2 ab = *reinterpret_cast<const float2*>(P.ab + (w.n * P.G + gr.g[i]) * 2);
+            c1[i] = k.rstd[i] * k.gamma[i];
+            c2[i] = -k.rstd[i] * ab.y;
+            c3[i] = -k.rstd[i] * ab.x;
+            if constexpr (DT != Y5M_F32) {
+                c2[i] *= k.rstd[i];
+                c3[i] = fmaf(-c2[i], k.mean[i], c3[i]);
+            }
+        }
+    }
+    auto finish = [&](const GnKept<DT, FMT>& kept, const Raw8<DT>& graw, T* to) __attribute__((always_inline)) {
+        float v[8], g[8];
+        gn_kept_values<DT, FMT>(kept, v);
+        unpack8<DT>(graw, g);
+        grad.template operator()<SILU>(v, g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[i] = fmaf(c1[i], g[i], fmaf(c2[i], v[i], c3[i]));
+        store8<DT, AL>(to, w.nv, g);
+    };
+    int r = w.r0 + w.lr;
+    GnCursor<DT, AL, FMT> at(P, w, r, static_cast<const T*>(P.dz) + w.n * P.zn + w.c);
+    T* op = static_cast<T*>(P.out) + w.n * P.on + (int64_t)r * P.orow + w.c;
+    const int64_t ostep = (int64_t)P.RP * P.orow;
+    for (; r + P.RP < w.r1; r += 2 * P.RP) {
+        GnKept<DT, FMT> kept[2];
+        Raw8<DT> graw[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) at.next(kept[u], graw[u]);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            finish(kept[u], graw[u], op);
+            op += ostep;
+        }
+    }
+    if (r < w.r1) {
+        GnKept<DT, FMT> kept;
+        Raw8<DT> graw;
+        at.next(kept, graw);
+        finish(kept, graw, op);
+    }
+}
+
+template <int DT, int AL, int FMT>
+__global__ __launch_bounds__(GN_THREADS) void gn_bwd_apply_kernel(const GnParams P) {
+    const GnPlace w = gn_place<true>(P, P.arpc);
+    if (w.n < 0 || !w.in) return;
+    if (P.act == Y5M_ACT_SILU) gn_bwd_rows<DT, AL, FMT, true>(P, w);
+    else gn_bwd_rows<DT, AL, FMT, false>(P, w);
+}
+
+// ---- held -------------------------------------------------------------------------------------------------------------------------
+// A workgroup of up to 512 threads (256 registers each) holds a slice of `sc` channels (whole groups; whole 32-channel blocks where the 8-bit form is
+// written) of one sample: NR row pieces per thread, RP rows side by side, two plain passes over registers for mean and variance.
+// Slices of a sample follow each other on one XCD (the hardware deals workgroups round the 8 XCDs): a row's cache lines, which several
+// slices share, are fetched once.
+#define GN_HELD_THREADS 512
+#ifndef GN_HELD_MAX
+#define GN_HELD_MAX (8ll << 20)
+#endif
+
+struct GnSlice { int64_t n; int c0, nc, lr, lc, c, nv; bool in; };
+__device__ __forceinline__ GnSlice gn_slice(const GnParams& P) {
+    const unsigned q8 = gridDim.x >> 3, r8 = gridDim.x & 7, xcd = blockIdx.x & 7;
+    const unsigned b = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + (blockIdx.x >> 3);
+    GnSlice w;
+    w.n = b / (unsigned)P.slices;
+    w.c0 = (int)(b - (unsigned)w.n * (unsigned)P.slices) * P.sc;
+    w.nc = P.C - w.c0 < P.sc ? P.C - w.c0 : P.sc;
+    w.lr = (int)threadIdx.x / P.ct;
+    w.lc = (int)threadIdx.x - w.lr * P.ct;
+    w.c = w.c0 + w.lc * 8;
+    w.nv = w.c0 + w.nc - w.c;
+    w.in = w.lr < P.RP && w.nv > 0;
+    return w;
+}
+// NS sums of 8 channels per thread -> tot[which][channel of the slice] in LDS. red: NS * 8 * threads floats, sub: threads floats,
+// tot: NS * sc floats
+template <int NS> __device__ __forceinline__ void gn_slice_sums(const GnParams& P, const GnSlice& w, const float* v, float* red, float* sub, float* tot) {
+    const int T = (int)blockDim.x, wd = P.ct * 8, cols = NS * wd;
+    __syncthreads();
+    if (w.in) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) red[w.lr * cols + s * wd + w.lc * 8 + k] = v[s * 8 + k];
+    }
+    __syncthreads();
+    const int rows = P.RP < P.S ? P.RP : P.S, parts = T / cols > 0 ? T / cols : 1;
+    for (int j = threadIdx.x; j < cols * parts; j += T) {
+        const int part = j / cols, c = j - part * cols;
+        float a = 0.f;
+        for (int r = part; r < rows; r += parts) a += red[r * cols + c];
+        if (parts > 1) sub[j] = a;
+        else tot[c] = a;
+    }
+    __syncthreads();
+    if (parts > 1) {
+        for (int c = threadIdx.x; c < cols; c += T) {
+            float a = 0.f;
+            for (int p = 0; p < parts; ++p) a += sub[p * cols + c];
+            tot[c] = a;
+        }
+        __syncthreads();
+    }
+}
+// f(group of the slice, sum over its channels of val(channel of the slice, i) in f64), one wave per group; f in lane 0
+template <int NV, typename V, typename F> __device__ __forceinline__ void gn_slice_groups(const GnParams& P, const GnSlice& w, V val, F f) {
+    const int lane = threadIdx.x & 63, groups = w.nc / P.D;
+    for (int g = threadIdx.x >> 6; g < groups; g += (int)blockDim.x >> 6) {
+        double a[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) a[i] = 0.0;
+        for (int d = lane; d < P.D; d += 64)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) a[i] += val(g * P.D + d, i);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) a[i] = gn_wave_sum(a[i]);
+        if (lane == 0) f(g, a);
+    }
+}
+
+template <int DT, int AL, int FMT, int NR>
+__global__ __launch_bounds__(GN_HELD_THREADS) void gn_held_kernel(const GnParams P) {
+    typedef typename RowElem<DT>::T T;
+    extern __shared__ __attribute__((aligned(16))) float lds[];
+    float *red = lds, *sub = red + 16 * blockDim.x, *tot = sub + blockDim.x, *gm = tot + P.ct * 16, *gr = gm + P.ct * 8;
+    const GnSlice w = gn_slice(P);
+    const T* b = static_cast<const T*>(P.x) + w.n * P.xn + (w.in ? w.c : w.c0);
+    const int nvl = w.in ? w.nv : w.nc, lr = w.lr < P.RP ? w.lr : 0;
+    Raw8<DT> raw[NR];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+        const int r = lr + i * P.RP;
+        raw[i] = load_raw8<DT, AL>(b + (int64_t)(r < P.S ? r : P.S - 1) * P.xr, nvl);
+    }
+    const double K = (double)P.S * (double)P.D;
+    float a[16], m[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) a[k] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+        const bool ok = lr + i * P.RP < P.S;
+        float v[8];
+        unpack8<DT>(raw[i], v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) a[k] += ok ? v[k] : 0.f;
+    }
+    gn_slice_sums<1>(P, w, a, red, sub, tot);
+    gn_slice_groups<1>(P, w, [&](int c, int) __attribute__((always_inline)) { return (double)tot[c]; },
+                       [&](int g, const double* s) __attribute__((always_inline)) { gm[g] = (float)(s[0] / K); });
+    __syncthreads();
+    const GnGroups gi = gn_groups(P, w.in ? w.lc * 8 : 0);         // (groups of the slice)
+    const int glast = w.nc / P.D - 1;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) m[k] = gm[gi.g[k] < glast ? gi.g[k] : glast];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) a[k] = 0.f;
+    // about that mean: the squares, and the rest of the mean (what the first sum's rounding lost)
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+        const bool ok = lr + i * P.RP < P.S;
+        float v[8];
+        unpack8<DT>(raw[i], v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float d = ok ? v[k] - m[k] : 0.f;
+            a[k] += d;
+            a[8 + k] = fmaf(d, d, a[8 + k]);
+        }
+    }
+    gn_slice_sums<2>(P, w, a, red, sub, tot);
+    const int wd = P.ct * 8;
+    gn_slice_groups<2>(P, w, [&](int c, int i) __attribute__((always_inline)) { return (double)tot[i * wd + c]; }, [&](int g, const double* s) __attribute__((always_inline)) {
+        const double off = s[0] / K, var = s[1] / K - off * off;
+        const float mean = (float)((double)gm[g] + off), rs = (float)(1.0 / sqrt((var > 0.0 || var != var ? var : 0.0) + (double)P.eps));
+        gm[g] = mean;
+        gr[g] = rs;
+        const int64_t ng = w.n * P.G + w.c0 / P.D + g;
+        P.mean[ng] = mean;
+        P.rstd[ng] = rs;
+    });
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 8; ++k) m[k] = gm[gi.g[k] < glast ? gi.g[k] : glast];
+    GnAffine<DT> af;
+    {
+        GnCoef k;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            k.mean[i] = m[i];
+            k.rstd[i] = gr[gi.g[i] < glast ? gi.g[i] : glast];
+            const int c = w.in && i < w.nv ? w.c + i : w.c0;
+            k.gamma[i] = P.gamma ? P.gamma[c] : 1.0f;
+            k.beta[i] = P.beta ? P.beta[c] : 0.0f;
+        }
+        af.set(k);
+    }
+    const bool silu = P.act == Y5M_ACT_SILU;
+    T* o = static_cast<T*>(P.out) + w.n * P.on + w.c;
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+        const int r = lr + i * P.RP;
+        const bool live = w.in && r < P.S;
+        float v[8], z[8];
+        unpack8<DT>(raw[i], v);
+        if constexpr (FMT != Y5M_KEEP_NONE) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) z[k] = w.in ? v[k] : 0.f;
+            unsigned sb;
+            const act8_u32x2 q = act8_encode8<FMT, DT>(z, sb);
+            if (live) {
+                const int64_t row = w.n * P.S + r;
+                *reinterpret_cast<act8_u32x2*>(P.q + row * P.ldq + w.c) = q;
+                if ((w.lc & 3) == 0) P.scale[row * P.CB + (w.c >> 5)] = (uint8_t)sb;
+            }
+        }
+        if (live) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float t = af(v[k], k);
+                z[k] = silu ? t * gn_sigmoid<DT>(t) : t;
+            }
+            store8<DT, AL>(o + (int64_t)r * P.orow, w.nv, z);
+        }
+    }
+}
+
+template <int DT, int AL, int FMT, int NR>
+__global__ __launch_bounds__(GN_HELD_THREADS) void gn_bwd_held_kernel(const GnParams P) {
+    typedef typename RowElem<DT>::T T;
+    extern __shared__ __attribute__((aligned(16))) float lds[];
+    float *red = lds, *sub = red + 16 * blockDim.x, *tot = sub + blockDim.x, *gA = tot + P.ct * 16, *gB = gA + P.ct * 8;
+    const GnSlice w = gn_slice(P);
+    const int lr = w.lr < P.RP ? w.lr : 0;
+    GnPlace at;                                                    // where gn_kept reads
+    at.n = w.n;
+    at.c = w.in ? w.c : w.c0;
+    at.nv = w.in ? w.nv : w.nc;
+    at.piece = at.c >> 3;
+    const T* d = static_cast<const T*>(P.dz) + w.n * P.zn + at.c;
+    GnKept<DT, FMT> kept[NR];
+    Raw8<DT> graw[NR];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+        const int r = lr + i * P.RP < P.S ? lr + i * P.RP : P.S - 1;
+        kept[i] = gn_kept<DT, AL, FMT>(P, at, r);
+        graw[i] = load_raw8<DT, AL>(d + (int64_t)r * P.zr, at.nv);
+    }
+    const GnGroups gi = gn_groups(P, w.in ? w.lc * 8 : 0);
+    const int glast = w.nc / P.D - 1;
+    GnCoef k;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int c = w.in && i < w.nv ? w.c + i : w.c0;
+        const int64_t ng = w.n * P.G + w.c0 / P.D + (gi.g[i] < glast ? gi.g[i] : glast);
+        k.mean[i] = P.mean[ng];
+        k.rstd[i] = P.rstd[ng];
+        k.gamma[i] = P.gamma ? P.gamma[c] : 1.0f;
+        k.beta[i] = P.beta ? P.beta[c] : 0.0f;
+    }
+    float c1[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c1[i] = k.rstd[i];
+    gn_coef_xhat<DT>(k);
+    const bool silu = P.act == Y5M_ACT_SILU;
+    auto grad = [&](const GnKept<DT, FMT>& kp, const Raw8<DT>& gw, float* xh, float* dt) __attribute__((always_inline)) {
+        gn_kept_values<DT, FMT>(kp, xh);
+        unpack8<DT>(gw, dt);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            xh[i] = gn_xhat<DT>(xh[i], k, i);
+            dt[i] *= gn_act_grad<DT>(silu, fmaf(xh[i], k.gamma[i], k.beta[i]));
+        }
+    };
+    float a[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) a[i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+        if (lr + i * P.RP < P.S) {
+            float xh[8], dt[8];
+            grad(kept[i], graw[i], xh, dt);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                a[j] += dt[j];
+                a[8 + j] = fmaf(dt[j], xh[j], a[8 + j]);
+            }
+        }
+    }
+    gn_slice_sums<2>(P, w, a, red, sub, tot);
+    const int wd = P.ct * 8;
+    for (int c = threadIdx.x; c < w.nc; c += (int)blockDim.x) {
+        *reinterpret_cast<float2*>(P.nc + ((size_t)w.n * P.C + w.c0 + c) * 2) = make_float2(tot[c], tot[wd + c]);
+        if (P.gamma) {
+            tot[c] *= P.gamma[w.c0 + c];
+            tot[wd + c] *= P.gamma[w.c0 + c];
+        }
+    }
+    __syncthreads();
+    const double K = (double)P.S * (double)P.D;
+    gn_slice_groups<2>(P, w, [&](int c, int i) __attribute__((always_inline)) { return (double)tot[i * wd + c]; }, [&](int g, const double* s) __attribute__((always_inline)) {
+        gA[g] = (float)(s[0] / K);
+        gB[g] = (float)(s[1] / K);
+    });
+    __syncthreads();
+    // dx = r gamma dt - r A - r B xhat = c1 dt + (c2 xhat + c3)
+    float c2[8], c3[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int g = gi.g[i] < glast ? gi.g[i] : glast;
+        c2[i] = -c1[i] * gB[g];
+        c3[i] = -c1[i] * gA[g];
+        c1[i] *= k.gamma[i];
+    }
+    T* o = static_cast<T*>(P.out) + w.n * P.on + w.c;
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+        const int r = lr + i * P.RP;
+        if (w.in && r < P.S) {
+            float xh[8], dt[8];
+            grad(kept[i], graw[i], xh, dt);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) dt[j] = fmaf(c1[j], dt[j], fmaf(c2[j], xh[j], c3[j]));
+            store8<DT, AL>(o + (int64_t)r * P.orow, w.nv, dt);
+        }
+    }
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------------------
 static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// column tiles of at most GN_THREADS pieces; row chunks so that about 4096 workgroups run and a thread still has 8 rows where there are
-static void gn_geometry(GnParams& P, bool quads) {
+// split: column tiles of at most GN_THREADS pieces; row chunks of 16 rows a thread in the reduce pass (whose sums are then joined), of 8
+// in the apply pass (short workgroups: 10000 of them stream at 6 TB/s, 2048 long ones at 5). 8 / 16, 12 / 12, 24 / 24 and 16 / 48 were 2 to
+// 9 % slower over the 40 x 40, 80 x 80 and 160 x 160 training steps at batch 64. At most 65536 chunks in all, so that the sums stay small
+// against the rows.
+#define GN_ROWS 16
+#define GN_APPLY_ROWS 8
+static void gn_geometry(GnParams& P, bool quads, int rows, int arows) {
     P.CB = (P.C + 31) / 32;
     P.CV = quads ? P.CB * 4 : (P.C + 7) / 8;
     P.tiles = (int)ceil_div(P.CV, GN_THREADS);
     P.ct = (int)ceil_div(P.CV, P.tiles);
     if (quads) P.ct = (P.ct + 3) / 4 * 4;
     P.RP = GN_THREADS / P.ct;
-    const int64_t most = ceil_div(P.S, (int64_t)P.RP * 8), want = ceil_div(4096, P.N * P.tiles);
-    int64_t chunks = want < most ? want : most;
-    if (chunks < 1) chunks = 1;
-    P.rpc = (int)ceil_div(ceil_div(P.S, chunks), P.RP) * P.RP;
-    P.chunks = (int)ceil_div(P.S, P.rpc);
+    auto cut = [&](int rows, int& chunks, int& rpc) {
+        int64_t c = ceil_div(P.S, (int64_t)P.RP * rows), cap = ceil_div(65536, P.N);
+        if (c > cap) c = cap;
+        rpc = (int)(ceil_div(ceil_div(P.S, c), P.RP) * P.RP);
+        chunks = (int)ceil_div(P.S, rpc);
+    };
+    cut(rows, P.chunks, P.rpc);
+    cut(arows, P.achunks, P.arpc);
+    P.ctm = gn_magic(P.ct);
 }
+
+// held: threads and rows per thread that hold a slice, NR = 0 where it does not fit. `nrs`: the row counts that are compiled, ascending
+struct GnHeld { int threads, nr; };
+static GnHeld gn_held(GnParams& P, bool blocks, const int* nrs) {
+    int a = P.D, b = blocks ? 32 : 8;
+    while (b) { const int t = a % b; a = b; b = t; }               // gcd
+    const int64_t lcm = (int64_t)P.D / a * (blocks ? 32 : 8);
+    const int unit = lcm < P.C ? (int)lcm : P.C, units = (int)ceil_div(P.C, unit);
+    auto pieces = [&](int sc) { const int p = (sc + 7) / 8; return blocks ? (p + 3) / 4 * 4 : p; };
+    auto fit = [&](int k) {
+        GnHeld h = {0, 0};
+        const int sc = (int64_t)unit * k < P.C ? unit * k : P.C, ct = pieces(sc);
+        for (int t = 256; t <= GN_HELD_THREADS; t *= 2) {
+            if (ct > t) continue;
+            const int64_t need = ceil_div(P.S, t / ct);
+            for (int i = 0; nrs[i]; ++i) {
+                if (need > nrs[i]) continue;
+                h.threads = t;
+                h.nr = nrs[i];
+                return h;
+            }
+        }
+        return h;
+    };
+    // wider slices (longer runs of a row, fewer idle threads) while 512 workgroups remain
+    int k = 1;
+    GnHeld h = fit(1);
+    while (h.nr && k < units && P.N * ceil_div(units, k + 1) >= 512 && (int64_t)P.S * pieces(unit * k) < 2048) {
+        const GnHeld w = fit(k + 1);
+        if (!w.nr) break;
+        h = w;
+        ++k;
+    }
+    if (h.nr == 0 || P.N * P.S * P.C > GN_HELD_MAX) return {0, 0};
+    P.sc = (int64_t)unit * k < P.C ? unit * k : P.C;
+    P.slices = (int)ceil_div(P.C, P.sc);
+    P.ct = pieces(P.sc);
+    P.RP = h.threads / P.ct;
+    P.CB = (P.C + 31) / 32;
+    if (P.N * P.slices >= (1ll << 31)) h.nr = 0;
+    return h;
+}
+static const int GN_FWD_ROWS[] = {4, 12, 0}, GN_BWD_ROWS[2][3] = {{4, 12, 0}, {4, 0, 0}};       // (backward: 16 bits, f32)
 
 static int gn_check(int64_t N, int64_t S, int C, int G, int act, int dtype) {
     Y5M_REQUIRE(dtype == Y5M_F32 || dtype == Y5M_BF16 || dtype == Y5M_F16, "dtype");
     Y5M_REQUIRE(act == Y5M_ACT_NONE || act == Y5M_ACT_SILU, "activation");
     Y5M_REQUIRE(C > 0 && G > 0 && C % G == 0, "the groups must divide the channels");
-    Y5M_REQUIRE(N >= 0 && S >= 0 && S < (1ll << 30) && N < (1ll << 30), "sizes");
+    Y5M_REQUIRE(N >= 0 && S >= 0 && S < (1ll << 30) && N < (1ll << 30) && C < (1 << 16), "sizes");
     return Y5M_OK;
 }
 static void gn_sizes(GnParams& P, int64_t N, int64_t S, int C, int G) {
-    P.N = N; P.S = (int)S; P.C = C; P.G = G; P.D = C / G;
+    P.N = N; P.S = (int)S; P.C = C; P.G = G; P.D = C / G; P.dm = gn_magic(P.D);
 }
 
 extern "C" size_t y5m_gn_act_workspace_bytes(int64_t N, int64_t S, int C, int G) {
-    if (N <= 0 || S <= 0 || C <= 0 || G <= 0 || C % G || S >= (1ll << 30)) return 0;
+    if (N <= 0 || S <= 0 || C <= 0 || G <= 0 || C % G || S >= (1ll << 30) || N >= (1ll << 30)) return 0;
     GnParams P = {};
     gn_sizes(P, N, S, C, G);
-    gn_geometry(P, true);
+    gn_geometry(P, true, GN_ROWS, GN_APPLY_ROWS);
     const int64_t a = P.chunks;
-    gn_geometry(P, false);
-    return (size_t)(N * (a > P.chunks ? a : P.chunks)) * 2 * C * sizeof(float);
+    gn_geometry(P, false, GN_ROWS, GN_APPLY_ROWS);
+    return (size_t)N * (size_t)(a > P.chunks ? a : P.chunks) * 2 * C * sizeof(float);
 }
 
 #define GN_DT(GO)                                                                    \
@@ -498,7 +1079,49 @@ extern "C" size_t y5m_gn_act_workspace_bytes(int64_t N, int64_t S, int C, int G)
         else if (dtype == Y5M_BF16) GO(Y5M_BF16);                                    \
         else GO(Y5M_F16);                                                            \
     } while (0)
-#define GN_LAUNCH(K, blocks) hipLaunchKernelGGL(K, dim3((unsigned)(blocks)), dim3(GN_THREADS), 0, y5m_stream(stream), P)
+#define GN_LAUNCH(K, blocks) hipLaunchKernelGGL(K, dim3((unsigned)(blocks)), dim3(GN_THREADS), 0, st, P)
+
+// a grid of (x, samples): the samples folded over y and z
+static dim3 gn_grid(int64_t x, int64_t N) {
+    const int64_t y = N < 32768 ? N : 32768;
+    return dim3((unsigned)x, (unsigned)y, (unsigned)ceil_div(N, y));
+}
+#define GN_LAUNCH2(K, x) hipLaunchKernelGGL(K, gn_grid((int64_t)(x) * P.tiles, P.N), dim3(GN_THREADS), 0, st, P)
+#define GN_LIMITS Y5M_REQUIRE((int64_t)P.chunks * P.tiles < (1ll << 31) && P.N * P.G < (1ll << 31), "too many workgroups")
+
+template <int DT, int AL, int FMT> static int gn_fwd_split(GnParams& P, hipStream_t st) {
+    gn_geometry(P, FMT != Y5M_KEEP_NONE, GN_ROWS, GN_APPLY_ROWS);
+    GN_LIMITS;
+    GN_LAUNCH2((gn_stats_kernel<DT, AL>), P.chunks);
+    GN_LAUNCH(gn_stats_join_kernel, P.N * P.G);
+    if constexpr (AL) {
+        if (rows_past_caches(P.N * P.S, P.C, DT)) GN_LAUNCH2((gn_apply_kernel<DT, 2, FMT>), P.achunks);
+        else GN_LAUNCH2((gn_apply_kernel<DT, 1, FMT>), P.achunks);
+    } else {
+        GN_LAUNCH2((gn_apply_kernel<DT, 0, FMT>), P.achunks);
+    }
+    Y5M_CHECK_LAUNCH("gn_apply_kernel");
+    return Y5M_OK;
+}
+// LDS above 64 KB has to be asked for, once per kernel
+#define GN_HELD_LAUNCH(K, lds)                                                                                                   \
+    do {                                                                                                                         \
+        static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(K), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024); \
+        if (e != hipSuccess) { y5m_set_error("%s: LDS refused", #K); return Y5M_ELAUNCH; }                                       \
+        hipLaunchKernelGGL(K, dim3((unsigned)(P.N * P.slices)), dim3(h.threads), lds, st, P);                                    \
+    } while (0)
+template <int DT, int AL, int FMT> static int gn_fwd(GnParams& P, hipStream_t st) {
+    const GnHeld h = gn_held(P, FMT != Y5M_KEEP_NONE, GN_FWD_ROWS);
+    if (h.nr == 0) return gn_fwd_split<DT, AL, FMT>(P, st);
+    const int lds = (17 * h.threads + 4 * P.ct * 8) * (int)sizeof(float);
+    if (h.nr == 4) GN_HELD_LAUNCH((gn_held_kernel<DT, AL, FMT, 4>), lds);
+    else GN_HELD_LAUNCH((gn_held_kernel<DT, AL, FMT, 12>), lds);
+    Y5M_CHECK_LAUNCH("gn_held_kernel");
+    return Y5M_OK;
+}
+template <int DT, int AL> static int gn_fwd_fmt(GnParams& P, int fmt, hipStream_t st) {
+    return fmt == Y5M_KEEP_NONE ? gn_fwd<DT, AL, Y5M_KEEP_NONE>(P, st) : fmt == Y5M_KEEP_E4M3 ? gn_fwd<DT, AL, Y5M_KEEP_E4M3>(P, st) : gn_fwd<DT, AL, Y5M_KEEP_INT8>(P, st);
+}
 
 extern "C" int y5m_gn_act(const void* x, int64_t x_batch_stride, int64_t x_row_stride, const float* gamma, const float* beta, int64_t N, int64_t S,
                           int C, int G, float eps, int act, void* z, int64_t z_batch_stride, int64_t z_row_stride, float* mean, float* rstd,
@@ -511,34 +1134,54 @@ extern "C" int y5m_gn_act(const void* x, int64_t x_batch_stride, int64_t x_row_s
     Y5M_REQUIRE(z != x || (z_batch_stride == x_batch_stride && z_row_stride == x_row_stride), "in place needs equal strides");
     Y5M_REQUIRE((S == 1 || z_row_stride >= C) && (N == 1 || z_batch_stride >= (S - 1) * z_row_stride + C), "rows of the output overlap");
     if (fmt != Y5M_KEEP_NONE) Y5M_REQUIRE(q && scale && ldq >= C && ldq % 8 == 0 && ((uintptr_t)q & 7) == 0, "8-bit form: ldq % 8 == 0, at least C, codes 8-byte aligned");
-    Y5M_REQUIRE(ws && ws_bytes >= y5m_gn_act_workspace_bytes(N, S, C, G), "workspace too small");
+    Y5M_REQUIRE(ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= y5m_gn_act_workspace_bytes(N, S, C, G), "workspace too small or not 16-byte aligned");
     GnParams P = {};
     gn_sizes(P, N, S, C, G);
     P.x = x; P.out = z; P.gamma = gamma; P.beta = beta; P.mean = mean; P.rstd = rstd; P.eps = eps; P.act = act;
     P.xn = x_batch_stride; P.xr = x_row_stride; P.on = z_batch_stride; P.orow = z_row_stride;
     P.q = static_cast<uint8_t*>(q); P.scale = static_cast<uint8_t*>(scale); P.ldq = ldq;
     P.part = static_cast<float*>(ws);
-    gn_geometry(P, fmt != Y5M_KEEP_NONE);
-    Y5M_REQUIRE(P.N * P.chunks * P.tiles < (1ll << 31) && P.N * P.G < (1ll << 31), "too many workgroups");
     const bool al = rows_aligned16(x, x_batch_stride, x_row_stride, N, S, C, dtype) && rows_aligned16(z, z_batch_stride, z_row_stride, N, S, C, dtype);
-    const int64_t blocks = P.N * P.chunks * P.tiles;
-#define GO(DT)                                                                                                                   \
-    do {                                                                                                                         \
-        if (al) GN_LAUNCH((gn_stats_kernel<DT, true>), blocks); else GN_LAUNCH((gn_stats_kernel<DT, false>), blocks);            \
-        GN_LAUNCH((gn_stats_join_kernel<DT>), ceil_div(P.N * P.G, GN_THREADS / 64));                                             \
-        if (fmt == Y5M_KEEP_NONE) { if (al) GN_LAUNCH((gn_apply_kernel<DT, true, Y5M_KEEP_NONE>), blocks); else GN_LAUNCH((gn_apply_kernel<DT, false, Y5M_KEEP_NONE>), blocks); } \
-        else if (fmt == Y5M_KEEP_E4M3) { if (al) GN_LAUNCH((gn_apply_kernel<DT, true, Y5M_KEEP_E4M3>), blocks); else GN_LAUNCH((gn_apply_kernel<DT, false, Y5M_KEEP_E4M3>), blocks); } \
-        else { if (al) GN_LAUNCH((gn_apply_kernel<DT, true, Y5M_KEEP_INT8>), blocks); else GN_LAUNCH((gn_apply_kernel<DT, false, Y5M_KEEP_INT8>), blocks); } \
-    } while (0)
+    hipStream_t st = y5m_stream(stream);
+#define GO(DT) rc = al ? gn_fwd_fmt<DT, true>(P, fmt, st) : gn_fwd_fmt<DT, false>(P, fmt, st)
     GN_DT(GO);
 #undef GO
-    Y5M_CHECK_LAUNCH("gn_act");
-    return Y5M_OK;
+    return rc;
 }
 
 extern "C" size_t y5m_gn_act_bwd_workspace_bytes(int64_t N, int64_t S, int C, int G) {
-    if (N <= 0 || S <= 0 || C <= 0 || G <= 0 || C % G || S >= (1ll << 30)) return 0;
+    if (N <= 0 || S <= 0 || C <= 0 || G <= 0 || C % G || S >= (1ll << 30) || N >= (1ll << 30)) return 0;
     return y5m_gn_act_workspace_bytes(N, S, C, G) + ((size_t)N * 2 * C + (size_t)N * G * 2) * sizeof(float);
+}
+
+template <int DT, int AL, int FMT> static int gn_bwd(GnParams& P, hipStream_t st) {
+    const GnHeld h = gn_held(P, false, GN_BWD_ROWS[DT == Y5M_F32]);
+    if (h.nr) {
+        const int lds = (17 * h.threads + 4 * P.ct * 8) * (int)sizeof(float);
+        if (h.nr == 4) GN_HELD_LAUNCH((gn_bwd_held_kernel<DT, AL, FMT, 4>), lds);
+        else if constexpr (DT != Y5M_F32) GN_HELD_LAUNCH((gn_bwd_held_kernel<DT, AL, FMT, 12>), lds);
+        Y5M_CHECK_LAUNCH("gn_bwd_held_kernel");
+    } else {
+        gn_geometry(P, false, GN_ROWS, GN_APPLY_ROWS);
+            GN_LIMITS;
+        GN_LAUNCH2((gn_bwd_reduce_kernel<DT, AL, FMT>), P.chunks);
+        GN_LAUNCH(gn_bwd_join_kernel, P.N * P.G);
+        if constexpr (AL) {
+            if (rows_past_caches(P.N * P.S, P.C, DT)) GN_LAUNCH2((gn_bwd_apply_kernel<DT, 2, FMT>), P.achunks);
+            else GN_LAUNCH2((gn_bwd_apply_kernel<DT, 1, FMT>), P.achunks);
+        } else {
+            GN_LAUNCH2((gn_bwd_apply_kernel<DT, 0, FMT>), P.achunks);
+        }
+        Y5M_CHECK_LAUNCH("gn_bwd_apply_kernel");
+    }
+    if (P.dgamma || P.dbeta) {
+        GN_LAUNCH(gn_param_grad_kernel, (P.C + 15) / 16);
+        Y5M_CHECK_LAUNCH("gn_param_grad_kernel");
+    }
+    return Y5M_OK;
+}
+template <int DT, int AL> static int gn_bwd_fmt(GnParams& P, int fmt, hipStream_t st) {
+    return fmt == Y5M_KEEP_NONE ? gn_bwd<DT, AL, Y5M_KEEP_NONE>(P, st) : fmt == Y5M_KEEP_E4M3 ? gn_bwd<DT, AL, Y5M_KEEP_E4M3>(P, st) : gn_bwd<DT, AL, Y5M_KEEP_INT8>(P, st);
 }
 
 extern "C" int y5m_gn_act_bwd(const void* dz, int64_t dz_batch_stride, int64_t dz_row_stride, const void* x, int64_t x_batch_stride, int64_t x_row_stride,
@@ -555,40 +1198,25 @@ extern "C" int y5m_gn_act_bwd(const void* dz, int64_t dz_batch_stride, int64_t d
     }
     Y5M_REQUIRE(dz && dx && mean && rstd, "null pointer");
     Y5M_REQUIRE((S == 1 || dx_row_stride >= C) && (N == 1 || dx_batch_stride >= (S - 1) * dx_row_stride + C), "rows of the output overlap");
+    Y5M_REQUIRE(dx != dz || (dx_batch_stride == dz_batch_stride && dx_row_stride == dz_row_stride), "in place needs equal strides");
+    Y5M_REQUIRE(dx != x || (dx_batch_stride == x_batch_stride && dx_row_stride == x_row_stride), "in place needs equal strides");
     if (fmt == Y5M_KEEP_NONE) Y5M_REQUIRE(x, "the input, or its 8-bit form");
     else Y5M_REQUIRE(q && scale && ldq >= C && ldq % 8 == 0 && ((uintptr_t)q & 7) == 0, "8-bit form: ldq % 8 == 0, at least C, codes 8-byte aligned");
-    Y5M_REQUIRE(ws && ws_bytes >= y5m_gn_act_bwd_workspace_bytes(N, S, C, G), "workspace too small");
+    Y5M_REQUIRE(ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= y5m_gn_act_bwd_workspace_bytes(N, S, C, G), "workspace too small or not 16-byte aligned");
     GnParams P = {};
     gn_sizes(P, N, S, C, G);
     P.x = x; P.dz = dz; P.out = dx; P.gamma = gamma; P.beta = beta; P.mean = const_cast<float*>(mean); P.rstd = const_cast<float*>(rstd); P.act = act;
     P.xn = x_batch_stride; P.xr = x_row_stride; P.zn = dz_batch_stride; P.zr = dz_row_stride; P.on = dx_batch_stride; P.orow = dx_row_stride;
     P.q = static_cast<uint8_t*>(const_cast<void*>(q)); P.scale = static_cast<uint8_t*>(const_cast<void*>(scale)); P.ldq = ldq;
     P.dgamma = dgamma; P.dbeta = dbeta;
-    gn_geometry(P, false);
-    P.part = static_cast<float*>(ws);
-    P.nc = P.part + (size_t)P.N * P.chunks * 2 * C;
-    P.ab = P.nc + (size_t)P.N * 2 * C;
-    Y5M_REQUIRE(P.N * P.chunks * P.tiles + C < (1ll << 31) && P.N * P.G < (1ll << 31), "too many workgroups");
+    P.nc = static_cast<float*>(ws);
+    P.ab = P.nc + (size_t)N * 2 * C;
+    P.part = P.ab + (size_t)N * 2 * G;
     const bool al = rows_aligned16(dz, dz_batch_stride, dz_row_stride, N, S, C, dtype) && rows_aligned16(dx, dx_batch_stride, dx_row_stride, N, S, C, dtype) &&
                     (fmt != Y5M_KEEP_NONE || rows_aligned16(x, x_batch_stride, x_row_stride, N, S, C, dtype));
-    const int64_t blocks = P.N * P.chunks * P.tiles;
-    P.main_blocks = (unsigned)blocks;
-    const int64_t extra = (dgamma || dbeta) ? (C + 15) / 16 : 0;
-#define GO2(DT, FMT)                                                                                                             \
-    do {                                                                                                                         \
-        if (al) GN_LAUNCH((gn_bwd_reduce_kernel<DT, true, FMT>), blocks); else GN_LAUNCH((gn_bwd_reduce_kernel<DT, false, FMT>), blocks); \
-        GN_LAUNCH(gn_bwd_join_kernel, ceil_div(P.N * P.G, GN_THREADS / 64));                                                     \
-        if (al) GN_LAUNCH((gn_bwd_apply_kernel<DT, true, FMT>), blocks + extra); else GN_LAUNCH((gn_bwd_apply_kernel<DT, false, FMT>), blocks + extra); \
-    } while (0)
-#define GO(DT)                                                                                                                   \
-    do {                                                                                                                         \
-        if (fmt == Y5M_KEEP_NONE) GO2(DT, Y5M_KEEP_NONE);                                                                        \
-        else if (fmt == Y5M_KEEP_E4M3) GO2(DT, Y5M_KEEP_E4M3);                                                                   \
-        else GO2(DT, Y5M_KEEP_INT8);                                                                                             \
-    } while (0)
+    hipStream_t st = y5m_stream(stream);
+#define GO(DT) rc = al ? gn_bwd_fmt<DT, true>(P, fmt, st) : gn_bwd_fmt<DT, false>(P, fmt, st)
     GN_DT(GO);
 #undef GO
-#undef GO2
-    Y5M_CHECK_LAUNCH("gn_act_bwd");
-    return Y5M_OK;
+    return rc;
 }
