@@ -252,7 +252,8 @@ class _DeviceGuard:
     device = "cuda"
 
     def stream(self):
-        return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+        # the raw handle of torch.cuda.current_stream(), without building the Stream object (4 us of a small call)
+        return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
     def tensors(self, *tensors):
         for t in tensors:

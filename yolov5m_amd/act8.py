@@ -33,7 +33,7 @@ _HERE = contextlib.nullcontext()
 
 def on_device_of(t):
     """context in which launches go to t's device (its current stream), whatever the current device is"""
-    if t.is_cuda and t.device.index != torch.cuda.current_device():
+    if t.is_cuda and t.get_device() != torch.cuda.current_device():
         return torch.cuda.device(t.device)
     return _HERE
 
@@ -47,16 +47,16 @@ def same_device(first, **others):
 
 def rows_of(t, name):
     """(N, S, C, batch stride, row stride) of a channels-last (N, C, *spatial) tensor, strides in elements"""
-    if t.dim() < 2:
-        raise Y5MError(f"{name}: expected (N, C, *spatial), got shape {tuple(t.shape)}")
     if t.dtype not in DTYPES:
         raise Y5MError(f"{name}: float32, bfloat16 or float16, got {t.dtype}")
     shape, st = t.shape, t.stride()
+    if len(shape) < 2:
+        raise Y5MError(f"{name}: expected (N, C, *spatial), got shape {tuple(shape)}")
     n, c = shape[0], shape[1]
     if c == 0:
         raise Y5MError(f"{name}: no channels")
     s, row, pitch = 1, None, 0
-    for d in range(t.dim() - 1, 1, -1):
+    for d in range(len(shape) - 1, 1, -1):
         size = shape[d]
         s *= size
         if size == 1:
@@ -75,7 +75,13 @@ def rows_of(t, name):
 
 def empty_rows(shape, dtype, device):
     """an uninitialised (N, C, *spatial) tensor, dense and channels last"""
-    return torch.empty((shape[0], *shape[2:], shape[1]), dtype=dtype, device=device).movedim(-1, 1)
+    c = shape[1]
+    st, run = [1] * len(shape), c
+    for d in range(len(shape) - 1, 1, -1):
+        st[d] = run
+        run *= shape[d]
+    st[0] = run
+    return torch.empty_strided(shape, st, dtype=dtype, device=device)
 
 
 class Act8:

@@ -25,25 +25,50 @@ template <int DT> struct Raw8 { act8_u32x4 r[DT == Y5M_F32 ? 2 : 1]; };
 __device__ __forceinline__ float f16_to_f32(uint16_t h) { return (float)__builtin_bit_cast(y5m_f16, h); }
 __device__ __forceinline__ uint16_t f32_to_f16(float f) { return __builtin_bit_cast(uint16_t, (y5m_f16)f); }
 
-// AL = 1: 16-byte pieces (the launcher checks base, strides and C). Else pieces that start at any element (unaligned vector loads where the
-// whole piece is inside the row: at 255 f32 channels a third of the time of element loads), a row's last piece by elements, the
-// channels >= nv as 0
+// AL = 1: 16-byte pieces (the launcher checks base, strides and C).
+// AL = 0: pieces that start at any element, C >= 8. A row's last piece (nv < 8) is read as the 8 elements that END with the row and
+// shifted down, zeros behind: every lane does the same, so the loads of an unrolled loop stay in flight together (a branch for the
+// short piece makes each load wait for the one before: 12 rows held in registers took 21 us of such waits).
+// AL = -1: C < 8, element by element; elements beyond the row are read as its last one and zeroed.
 template <int DT, int AL>
 __device__ __forceinline__ Raw8<DT> load_raw8(const typename RowElem<DT>::T* __restrict__ p, int nv) {
     Raw8<DT> w;
-    if constexpr (AL) {
+    if constexpr (AL > 0) {
         w.r[0] = *reinterpret_cast<const act8_u32x4*>(p);
         if constexpr (DT == Y5M_F32) w.r[1] = *reinterpret_cast<const act8_u32x4*>(p + 4);
-    } else if (nv >= 8) {
-        __builtin_memcpy(&w, p, sizeof(w));
-    } else if constexpr (DT == Y5M_F32) {
+    } else if constexpr (AL == 0) {
+        const int sh = nv < 8 ? 8 - nv : 0;
+        __builtin_memcpy(&w, p - sh, sizeof(w));
+        if constexpr (DT == Y5M_F32) {
+            unsigned v[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) w.r[k >> 2][k & 3] = k < nv ? __float_as_uint(p[k]) : 0u;
+            for (int k = 0; k < 8; ++k) v[k] = w.r[k >> 2][k & 3];
+#pragma unroll
+            for (int s = 4; s > 0; s >>= 1)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] = (sh & s) ? (k + s < 8 ? v[k + s < 8 ? k + s : 0] : 0u) : v[k];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) w.r[k >> 2][k & 3] = v[k];
+        } else {
+            unsigned v[5] = {w.r[0][0], w.r[0][1], w.r[0][2], w.r[0][3], 0u};
+#pragma unroll
+            for (int s = 4; s > 1; s >>= 1)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = (sh & s) ? (k + s / 2 < 4 ? v[k + s / 2 < 4 ? k + s / 2 : 0] : 0u) : v[k];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w.r[0][k] = (sh & 1) ? (v[k] >> 16) | (v[k + 1] << 16) : v[k];
+        }
     } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const unsigned lo = 2 * k < nv ? p[2 * k] : 0u, hi = 2 * k + 1 < nv ? p[2 * k + 1] : 0u;
-            w.r[0][k] = lo | (hi << 16);
+        for (int k = 0; k < 8; ++k) {
+            const typename RowElem<DT>::T e = p[k < nv ? k : nv - 1];
+            if constexpr (DT == Y5M_F32) {
+                w.r[k >> 2][k & 3] = k < nv ? __float_as_uint(e) : 0u;
+            } else {
+                const unsigned x = k < nv ? (unsigned)e : 0u;
+                if (k & 1) w.r[0][k >> 1] |= x << 16;
+                else w.r[0][k >> 1] = x;
+            }
         }
     }
     return w;
@@ -75,7 +100,7 @@ __device__ __forceinline__ void store8(typename RowElem<DT>::T* __restrict__ p, 
 #pragma unroll
         for (int k = 0; k < 4; ++k) w.r[0][k] = (unsigned)f32_to_f16(v[2 * k]) | ((unsigned)f32_to_f16(v[2 * k + 1]) << 16);
     }
-    if constexpr (AL) {
+    if constexpr (AL > 0) {
         act8_u32x4* q = reinterpret_cast<act8_u32x4*>(p);
 #pragma unroll
         for (int h = 0; h < (DT == Y5M_F32 ? 2 : 1); ++h) {
@@ -173,6 +198,8 @@ template <int FMT> __device__ __forceinline__ void act8_decode8(act8_u32x2 q, fl
     }
 }
 
+// host: the AL of kernels for these rows
+static inline int rows_mode(bool aligned, int C) { return aligned ? 1 : C >= 8 ? 0 : -1; }
 // host: may rows at p (batch stride sn, row stride sr, in elements) be read in 16-byte pieces?
 static inline bool rows_aligned16(const void* p, int64_t sn, int64_t sr, int64_t N, int64_t S, int C, int dtype) {
     const int per = dtype == Y5M_F32 ? 4 : 8;

@@ -129,7 +129,8 @@ static void act8_geometry(Act8Params& P) {
     } while (0)
 #define ACT8_D3(KERN, DT, FMT, NT)                                                                                                \
     do {                                                                                                                          \
-        if (!al) ACT8_GO((KERN<DT, FMT, 0>));                                                                                     \
+        if (al < 0) ACT8_GO((KERN<DT, FMT, -1>));                                                                                 \
+        else if (al == 0) ACT8_GO((KERN<DT, FMT, 0>));                                                                                     \
         else if (nt) ACT8_GO((KERN<DT, FMT, NT>));                                                                                \
         else ACT8_GO((KERN<DT, FMT, 1>));                                                                                         \
     } while (0)
@@ -149,7 +150,7 @@ extern "C" int y5m_act8_store(const void* x, int64_t x_batch_stride, int64_t x_r
         if (S == 1 && N > 1) P.sr = x_batch_stride;
         P.S = 0;
     }
-    const bool al = rows_aligned16(x, x_batch_stride, x_row_stride, N, S, C, dtype);
+    const int al = rows_mode(rows_aligned16(x, x_batch_stride, x_row_stride, N, S, C, dtype), C);
     const bool nt = false;
     ACT8_DISPATCH(act8_store_kernel, 1);
     Y5M_CHECK_LAUNCH("act8_store_kernel");
@@ -168,7 +169,7 @@ extern "C" int y5m_act8_load(const void* q, int ldq, const void* scale, int64_t 
     P.C = C; P.ldq = ldq;
     const bool nt = rows_past_caches(M, C, dtype);
     act8_geometry(P);
-    const bool al = rows_aligned16(x, 0, x_row_stride, 1, M, C, dtype);
+    const int al = rows_mode(rows_aligned16(x, 0, x_row_stride, 1, M, C, dtype), C);
     ACT8_DISPATCH(act8_load_kernel, 2);
     Y5M_CHECK_LAUNCH("act8_load_kernel");
     return Y5M_OK;

@@ -101,11 +101,11 @@ __device__ __forceinline__ void gn_join_rows(const float* v, float* red, const G
     const int wd = ct * 8, c0 = (w.piece - w.lc) * 8;
     float* red2 = red + GN_THREADS * 8;
     if (w.in) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            red[w.lr * wd + w.lc * 8 + k] = v[k];
-            red2[w.lr * wd + w.lc * 8 + k] = v[8 + k];
-        }
+        float4 *d = reinterpret_cast<float4*>(red + w.lr * wd + w.lc * 8), *d2 = reinterpret_cast<float4*>(red2 + w.lr * wd + w.lc * 8);
+        d[0] = make_float4(v[0], v[1], v[2], v[3]);
+        d[1] = make_float4(v[4], v[5], v[6], v[7]);
+        d2[0] = make_float4(v[8], v[9], v[10], v[11]);
+        d2[1] = make_float4(v[12], v[13], v[14], v[15]);
     }
     __syncthreads();
     const int parts = GN_THREADS / wd;
@@ -151,7 +151,8 @@ __device__ __forceinline__ void gn_join_rows(const float* v, float* red, const G
         f(c0 + j, a, b);
     }
 }
-__device__ __forceinline__ float* gn_part(const GnParams& P, const GnPlace& w) { return P.part + ((size_t)w.n * P.chunks + w.chunk) * 2 * P.C; }
+// (with a channel's chunks next to each other the join is 1 us shorter and the reduce pass, whose 8-byte stores then scatter, 3 to 8 longer)
+__device__ __forceinline__ float2* gn_part(const GnParams& P, const GnPlace& w, int c) { return reinterpret_cast<float2*>(P.part) + ((size_t)w.n * P.chunks + w.chunk) * P.C + c; }
 
 // ---- forward, split ---------------------------------------------------------------------------------------------------------------
 // Squares are summed about the chunk's first row: a chunk's mean and M2 = sum (x - p)^2 - (sum (x - p))^2 / R then cancel by at most a
@@ -159,7 +160,7 @@ __device__ __forceinline__ float* gn_part(const GnParams& P, const GnPlace& w) {
 template <int DT, int AL>
 __global__ __launch_bounds__(GN_THREADS) void gn_stats_kernel(const GnParams P) {
     typedef typename RowElem<DT>::T T;
-    __shared__ float red[GN_THREADS * 16];
+    __shared__ __attribute__((aligned(16))) float red[GN_THREADS * 16];
     const GnPlace w = gn_place<false>(P, P.rpc);
     if (w.n >= P.N) return;
     float a[16], pv[8];
@@ -198,7 +199,6 @@ __global__ __launch_bounds__(GN_THREADS) void gn_stats_kernel(const GnParams P) 
         }
     }
     // channel sums about the first row -> the chunk's mean and M2
-    float* dst = gn_part(P, w);
     const float R = (float)(w.r1 - w.r0);
     const T* first = static_cast<const T*>(P.x) + w.n * P.xn + (int64_t)w.r0 * P.xr;
     gn_join_rows(a, red, w, P.ct, P.RP, P.C, [&](int c, float s1, float s2) __attribute__((always_inline)) {
@@ -206,17 +206,18 @@ __global__ __launch_bounds__(GN_THREADS) void gn_stats_kernel(const GnParams P) 
         if constexpr (DT == Y5M_F32) pv = first[c];
         else if constexpr (DT == Y5M_BF16) pv = bf16_to_f32(first[c]);
         else pv = f16_to_f32(first[c]);
-        *reinterpret_cast<float2*>(dst + 2 * c) = make_float2(pv + s1 / R, s2 - s1 * s1 / R);
+        *gn_part(P, w, c) = make_float2(pv + s1 / R, s2 - s1 * s1 / R);
     });
 }
 
+__device__ __forceinline__ double gn_shfl_xor(double v, int o) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const unsigned lo = (unsigned)__shfl_xor((int)(unsigned)u, o, 64), hi = (unsigned)__shfl_xor((int)(unsigned)(u >> 32), o, 64);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
 __device__ __forceinline__ double gn_wave_sum(double v) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const uint64_t u = __builtin_bit_cast(uint64_t, v);
-        const unsigned lo = (unsigned)__shfl_xor((int)(unsigned)u, o, 64), hi = (unsigned)__shfl_xor((int)(unsigned)(u >> 32), o, 64);
-        v += __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-    }
+    for (int o = 32; o > 0; o >>= 1) v += gn_shfl_xor(v, o);
     return v;
 }
 // a workgroup's sum of NV doubles per thread, in a fixed order; every thread gets it
@@ -540,7 +541,7 @@ __device__ __forceinline__ void gn_bwd_sums(const GnParams& P, const GnPlace& w,
 
 template <int DT, int AL, int FMT>
 __global__ __launch_bounds__(GN_THREADS) void gn_bwd_reduce_kernel(const GnParams P) {
-    __shared__ float red[GN_THREADS * 16];
+    __shared__ __attribute__((aligned(16))) float red[GN_THREADS * 16];
     const GnPlace w = gn_place<false>(P, P.rpc);
     if (w.n >= P.N) return;
     float a[16];
@@ -551,8 +552,7 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_reduce_kernel(const GnParam
         if (P.act == Y5M_ACT_SILU) gn_bwd_sums<DT, AL, FMT, true>(P, w, gr, a);
         else gn_bwd_sums<DT, AL, FMT, false>(P, w, gr, a);
     }
-    float* dst = gn_part(P, w);
-    gn_join_rows(a, red, w, P.ct, P.RP, P.C, [&](int c, float s0, float s1) __attribute__((always_inline)) { *reinterpret_cast<float2*>(dst + 2 * c) = make_float2(s0, s1); });
+    gn_join_rows(a, red, w, P.ct, P.RP, P.C, [&](int c, float s0, float s1) __attribute__((always_inline)) { *gn_part(P, w, c) = make_float2(s0, s1); });
 }
 
 // channel sums of a sample and A, B of its groups, one workgroup per (sample, group)
@@ -736,9 +736,11 @@ template <int NS> __device__ __forceinline__ void gn_slice_sums(const GnParams& 
     __syncthreads();
     if (w.in) {
 #pragma unroll
-        for (int s = 0; s < NS; ++s)
-#pragma unroll
-            for (int k = 0; k < 8; ++k) red[w.lr * cols + s * wd + w.lc * 8 + k] = v[s * 8 + k];
+        for (int s = 0; s < NS; ++s) {
+            float4* d = reinterpret_cast<float4*>(red + w.lr * cols + s * wd + w.lc * 8);
+            d[0] = make_float4(v[s * 8], v[s * 8 + 1], v[s * 8 + 2], v[s * 8 + 3]);
+            d[1] = make_float4(v[s * 8 + 4], v[s * 8 + 5], v[s * 8 + 6], v[s * 8 + 7]);
+        }
     }
     __syncthreads();
     const int rows = P.RP < P.S ? P.RP : P.S, parts = T / cols > 0 ? T / cols : 1;
@@ -1020,16 +1022,13 @@ static GnHeld gn_held(GnParams& P, bool blocks, const int* nrs) {
     auto fit = [&](int k) {
         GnHeld h = {0, 0};
         const int sc = (int64_t)unit * k < P.C ? unit * k : P.C, ct = pieces(sc);
-        for (int t = 256; t <= GN_HELD_THREADS; t *= 2) {
-            if (ct > t) continue;
-            const int64_t need = ceil_div(P.S, t / ct);
-            for (int i = 0; nrs[i]; ++i) {
-                if (need > nrs[i]) continue;
+        for (int i = 0; nrs[i]; ++i)                               // (few rows a thread before few threads: what is serial is what counts)
+            for (int t = 256; t <= GN_HELD_THREADS; t *= 2) {
+                if (ct > t || ceil_div(P.S, t / ct) > nrs[i]) continue;
                 h.threads = t;
                 h.nr = nrs[i];
                 return h;
             }
-        }
         return h;
     };
     // wider slices (longer runs of a row, fewer idle threads) while 512 workgroups remain
@@ -1087,18 +1086,18 @@ static dim3 gn_grid(int64_t x, int64_t N) {
     return dim3((unsigned)x, (unsigned)y, (unsigned)ceil_div(N, y));
 }
 #define GN_LAUNCH2(K, x) hipLaunchKernelGGL(K, gn_grid((int64_t)(x) * P.tiles, P.N), dim3(GN_THREADS), 0, st, P)
-#define GN_LIMITS Y5M_REQUIRE((int64_t)P.chunks * P.tiles < (1ll << 31) && P.N * P.G < (1ll << 31), "too many workgroups")
+#define GN_LIMITS Y5M_REQUIRE((int64_t)P.achunks * P.tiles + P.C < (1ll << 31) && (int64_t)P.chunks * P.tiles < (1ll << 31) && P.N * P.G < (1ll << 31), "too many workgroups")
 
 template <int DT, int AL, int FMT> static int gn_fwd_split(GnParams& P, hipStream_t st) {
     gn_geometry(P, FMT != Y5M_KEEP_NONE, GN_ROWS, GN_APPLY_ROWS);
     GN_LIMITS;
     GN_LAUNCH2((gn_stats_kernel<DT, AL>), P.chunks);
     GN_LAUNCH(gn_stats_join_kernel, P.N * P.G);
-    if constexpr (AL) {
+    if constexpr (AL > 0) {
         if (rows_past_caches(P.N * P.S, P.C, DT)) GN_LAUNCH2((gn_apply_kernel<DT, 2, FMT>), P.achunks);
         else GN_LAUNCH2((gn_apply_kernel<DT, 1, FMT>), P.achunks);
     } else {
-        GN_LAUNCH2((gn_apply_kernel<DT, 0, FMT>), P.achunks);
+        GN_LAUNCH2((gn_apply_kernel<DT, AL, FMT>), P.achunks);
     }
     Y5M_CHECK_LAUNCH("gn_apply_kernel");
     return Y5M_OK;
@@ -1141,9 +1140,9 @@ extern "C" int y5m_gn_act(const void* x, int64_t x_batch_stride, int64_t x_row_s
     P.xn = x_batch_stride; P.xr = x_row_stride; P.on = z_batch_stride; P.orow = z_row_stride;
     P.q = static_cast<uint8_t*>(q); P.scale = static_cast<uint8_t*>(scale); P.ldq = ldq;
     P.part = static_cast<float*>(ws);
-    const bool al = rows_aligned16(x, x_batch_stride, x_row_stride, N, S, C, dtype) && rows_aligned16(z, z_batch_stride, z_row_stride, N, S, C, dtype);
+    const int al = rows_mode(rows_aligned16(x, x_batch_stride, x_row_stride, N, S, C, dtype) && rows_aligned16(z, z_batch_stride, z_row_stride, N, S, C, dtype), C);
     hipStream_t st = y5m_stream(stream);
-#define GO(DT) rc = al ? gn_fwd_fmt<DT, true>(P, fmt, st) : gn_fwd_fmt<DT, false>(P, fmt, st)
+#define GO(DT) rc = al > 0 ? gn_fwd_fmt<DT, 1>(P, fmt, st) : al == 0 ? gn_fwd_fmt<DT, 0>(P, fmt, st) : gn_fwd_fmt<DT, -1>(P, fmt, st)
     GN_DT(GO);
 #undef GO
     return rc;
@@ -1166,14 +1165,15 @@ template <int DT, int AL, int FMT> static int gn_bwd(GnParams& P, hipStream_t st
             GN_LIMITS;
         GN_LAUNCH2((gn_bwd_reduce_kernel<DT, AL, FMT>), P.chunks);
         GN_LAUNCH(gn_bwd_join_kernel, P.N * P.G);
-        if constexpr (AL) {
+        if constexpr (AL > 0) {
             if (rows_past_caches(P.N * P.S, P.C, DT)) GN_LAUNCH2((gn_bwd_apply_kernel<DT, 2, FMT>), P.achunks);
             else GN_LAUNCH2((gn_bwd_apply_kernel<DT, 1, FMT>), P.achunks);
         } else {
-            GN_LAUNCH2((gn_bwd_apply_kernel<DT, 0, FMT>), P.achunks);
+            GN_LAUNCH2((gn_bwd_apply_kernel<DT, AL, FMT>), P.achunks);
         }
         Y5M_CHECK_LAUNCH("gn_bwd_apply_kernel");
     }
+    // (as workgroups of the apply pass the parameters' gradients cost it more, in registers, than this launch)
     if (P.dgamma || P.dbeta) {
         GN_LAUNCH(gn_param_grad_kernel, (P.C + 15) / 16);
         Y5M_CHECK_LAUNCH("gn_param_grad_kernel");
@@ -1212,10 +1212,10 @@ extern "C" int y5m_gn_act_bwd(const void* dz, int64_t dz_batch_stride, int64_t d
     P.nc = static_cast<float*>(ws);
     P.ab = P.nc + (size_t)N * 2 * C;
     P.part = P.ab + (size_t)N * 2 * G;
-    const bool al = rows_aligned16(dz, dz_batch_stride, dz_row_stride, N, S, C, dtype) && rows_aligned16(dx, dx_batch_stride, dx_row_stride, N, S, C, dtype) &&
-                    (fmt != Y5M_KEEP_NONE || rows_aligned16(x, x_batch_stride, x_row_stride, N, S, C, dtype));
+    const int al = rows_mode(rows_aligned16(dz, dz_batch_stride, dz_row_stride, N, S, C, dtype) && rows_aligned16(dx, dx_batch_stride, dx_row_stride, N, S, C, dtype) &&
+                             (fmt != Y5M_KEEP_NONE || rows_aligned16(x, x_batch_stride, x_row_stride, N, S, C, dtype)), C);
     hipStream_t st = y5m_stream(stream);
-#define GO(DT) rc = al ? gn_bwd_fmt<DT, true>(P, fmt, st) : gn_bwd_fmt<DT, false>(P, fmt, st)
+#define GO(DT) rc = al > 0 ? gn_bwd_fmt<DT, 1>(P, fmt, st) : al == 0 ? gn_bwd_fmt<DT, 0>(P, fmt, st) : gn_bwd_fmt<DT, -1>(P, fmt, st)
     GN_DT(GO);
 #undef GO
     return rc;

@@ -42,8 +42,7 @@ def _param(t, c, name, x):
         raise Y5MError(f"{name}: a floating-point tensor, got {t.dtype}")
     if t.device != x.device:
         raise Y5MError(f"{name} is on {t.device}, expected {x.device}")
-    t = t.detach()
-    return t if t.dtype == torch.float32 and t.is_contiguous() else t.float().contiguous()
+    return t if t.dtype == torch.float32 and t.is_contiguous() else t.detach().float().contiguous()
 
 
 def _ptr(t):
@@ -68,20 +67,26 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="silu", keep
     w, b = _param(weight, c, "weight", x), _param(bias, c, "bias", x)
     L = _lib.lib()
     with on_device_of(x):
-        xd = x.detach()
         z = empty_rows(x.shape, x.dtype, x.device)
-        stat = torch.empty((2, n, groups), dtype=torch.float32, device=x.device)
         a = new_act8(x, keep) if keep in FORMATS else None
-        wsb = L.y5m_gn_act_workspace_bytes(n, s, c, groups)
-        ws = torch.empty(wsb, dtype=torch.uint8, device=x.device)
-        _lib.check(L.y5m_gn_act(xd.data_ptr(), sn, sr, _ptr(w), _ptr(b), n, s, c, groups, eps, _ACTS[act], z.data_ptr(), s * c, c,
-                                stat.data_ptr(), stat.data_ptr() + 4 * n * groups, a.q.data_ptr() if a else None, a.q.shape[1] if a else 0,
-                                a.scale.data_ptr() if a else None, FORMATS[keep] if a else 0, ws.data_ptr(), wsb, DTYPES[x.dtype],
+        # mean, rstd and the workspace in one allocation where nobody keeps the statistics
+        ng = n * groups
+        wsb, sb = L.y5m_gn_act_workspace_bytes(n, s, c, groups), (8 * ng + 255) // 256 * 256
+        if keep is None:
+            mem = torch.empty(sb + wsb, dtype=torch.uint8, device=x.device)
+            mean, ws = mem.data_ptr(), mem.data_ptr() + sb
+        else:
+            stat = torch.empty((2, n, groups), dtype=torch.float32, device=x.device)
+            mem = torch.empty(wsb, dtype=torch.uint8, device=x.device)
+            mean, ws = stat.data_ptr(), mem.data_ptr()
+        _lib.check(L.y5m_gn_act(x.data_ptr(), sn, sr, _ptr(w), _ptr(b), n, s, c, groups, eps, _ACTS[act], z.data_ptr(), s * c, c,
+                                mean, mean + 4 * ng, a.q.data_ptr() if a else None, a.q.shape[1] if a else 0,
+                                a.scale.data_ptr() if a else None, FORMATS[keep] if a else 0, ws, wsb, DTYPES[x.dtype],
                                 _lib.stream_ptr()), "y5m_gn_act")
     if keep is None:
         return z, None
     sv = GroupNormSaved()
-    sv.kept = a if a else xd
+    sv.kept = a if a else x.detach()
     sv.mean, sv.rstd, sv.groups, sv.act, sv.weight, sv.bias = stat[0], stat[1], groups, act, w, b
     return z, sv
 
