@@ -22,7 +22,7 @@ RULES = [
                 r'::\s*"s"\((\w+)\),\s*"v"\((\w+)\),\s*"s"\((\w+)\),\s*"s"\((\w+)\)\s*:\s*"memory"\);', re.S),
      r'emu_buffer_load_lds16(\3, \2, \4, \1);'),
     (re.compile(r'asm volatile\("s_memtime %0\\n\\ts_waitcnt lgkmcnt\(0\)"\s*:\s*"=s"\((\w+)\)\s*::\s*"memory"\);'), r'\1 = 0;'),
-    (re.compile(r'asm\(""\s*:\s*"\+v"\((\w+)\)\);'), r'asm("" : "+r"(\1));'),
+    (re.compile(r'asm( volatile)?\(""\s*:\s*"\+v"\((\w+)\)\);'), r'asm\1("" : "+r"(\2));'),
 ]
 
 

@@ -40,7 +40,7 @@ template <int DT, int PA, int PC> struct AwStage {
     static constexpr int AD = DT == Y5M_F32 ? PA : PA / 2;
     unsigned a[8][AD];
     unsigned q[8][PC / 4];
-    unsigned s[8];
+    unsigned s, s2;                          // scale bytes of row 8 g + (i & 7), blocks (i >> 3) and (i >> 3) + 2 of the tile
 };
 
 // n dwords at byte offset `off` of a buffer resource: zero beyond its last byte, in hardware
@@ -71,10 +71,17 @@ template <int DT, int PA, int PC, bool FAST> struct AwLoader {
     int n, c, g;
     bool nin, cin;
     __amdgpu_buffer_rsrc_t ry, rq, rs;
-    unsigned ao, qo, so, as;                 // byte offsets of row 8 g of the range, bytes from row to row of dY
-    __device__ __forceinline__ AwLoader(const AwParams& P_, int64_t m0_, int64_t m1_, int n_, int c_, int g_) : P(P_), m0(m0_), m1(m1_), n(n_), c(c_), g(g_) {
+    unsigned ao, qo, so, as;                 // byte offsets of row 8 g (scales: of this lane's row) of the range, bytes from row to row of dY
+    int sr, sb;                              // the row and block of the tile whose scale this lane fetches
+    bool sin, sin2;
+    __device__ __forceinline__ AwLoader(const AwParams& P_, int64_t m0_, int64_t m1_, int n_, int c_, int g_, int c0, int i16)
+        : P(P_), m0(m0_), m1(m1_), n(n_), c(c_), g(g_) {
         nin = n < P.N;
         cin = c < P.C;
+        sr = 8 * g + (i16 & 7);
+        sb = (c0 >> 5) + (i16 >> 3);
+        sin = sb < P.CB;
+        sin2 = PC == 8 && sb + 2 < P.CB;
         if constexpr (FAST) {
             as = (unsigned)(P.dr * (int64_t)sizeof(T));
             const unsigned rows = (unsigned)(m1 - m0);
@@ -83,7 +90,7 @@ template <int DT, int PA, int PC, bool FAST> struct AwLoader {
             rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(P.scale + m0 * P.CB), 0, rows * (unsigned)P.CB, 0x00020000);
             ao = nin ? (unsigned)(8 * g) * as + (unsigned)n * (unsigned)sizeof(T) : OOB;
             qo = cin ? (unsigned)(8 * g) * (unsigned)P.ldq + (unsigned)c : OOB;
-            so = cin ? (unsigned)(8 * g) * (unsigned)P.CB + ((unsigned)c >> 5) : OOB;
+            so = (unsigned)sr * (unsigned)P.CB + (unsigned)sb;
         }
     }
     __device__ __forceinline__ void load(AwStage<DT, PA, PC>& st, unsigned step) const {       // step: rows from m0
@@ -94,43 +101,52 @@ template <int DT, int PA, int PC, bool FAST> struct AwLoader {
             for (int j = 0; j < 8; ++j) {
                 aw_buffer<AD>(ry, a + (unsigned)j * as, st.a[j]);
                 aw_buffer<PC / 4>(rq, q + (unsigned)(j * P.ldq), st.q[j]);
-                st.s[j] = __builtin_amdgcn_raw_buffer_load_b8(rs, s + (unsigned)(j * P.CB), 0, 0);
             }
+            st.s = __builtin_amdgcn_raw_buffer_load_b8(rs, sin ? s : OOB, 0, 0);
+            if constexpr (PC == 8) st.s2 = __builtin_amdgcn_raw_buffer_load_b8(rs, sin2 ? s + 2 : OOB, 0, 0);
         } else {
-            // rows of unaligned pieces (the compiler's unaligned vector loads), a row's last piece by elements; P.S = 0: one distance
-            const bool whole = n + PA <= P.N;
+            // rows that start anywhere (the compiler's unaligned vector loads). A row's last piece is the PA values that END with the
+            // row, shifted down, so that no lane branches around a load; N < PA by elements. P.S = 0: the rows at one distance
+            const int sh = nin && n + PA > P.N ? n + PA - P.N : 0, nl = nin ? n - sh : 0;
+            const bool small = P.N < PA;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int64_t row = m0 + step + 8 * g + j;
                 const bool in = row < m1;
                 const int64_t r = in ? row : m0, nb = P.S ? r / P.S : 0;
-                const T* p = static_cast<const T*>(P.dy) + nb * P.dn + (r - nb * P.S) * P.dr + n;
-                if (whole) {
-                    __builtin_memcpy(st.a[j], p, sizeof(st.a[j]));
-                } else if constexpr (DT == Y5M_F32) {
+                const T* p = static_cast<const T*>(P.dy) + nb * P.dn + (r - nb * P.S) * P.dr;
+                T e[PA];
+                if (small) {
 #pragma unroll
-                    for (int k = 0; k < PA; ++k) st.a[j][k] = n + k < P.N ? __float_as_uint(p[k]) : 0u;
+                    for (int k = 0; k < PA; ++k) e[k] = p[n + k < P.N ? n + k : P.N - 1];
+                } else {
+                    __builtin_memcpy(e, p + nl, sizeof(e));
+#pragma unroll
+                    for (int s2 = PA / 2; s2 > 0; s2 >>= 1)
+#pragma unroll
+                        for (int k = 0; k + s2 < PA; ++k) e[k] = (sh & s2) ? e[k + s2] : e[k];
+                }
+                if constexpr (DT == Y5M_F32) {
+#pragma unroll
+                    for (int k = 0; k < PA; ++k) st.a[j][k] = in && n + k < P.N ? __float_as_uint(e[k]) : 0u;
                 } else {
 #pragma unroll
-                    for (int k = 0; k < PA / 2; ++k) {
-                        const unsigned lo = n + 2 * k < P.N ? p[2 * k] : 0u, hi = n + 2 * k + 1 < P.N ? p[2 * k + 1] : 0u;
-                        st.a[j][k] = lo | (hi << 16);
-                    }
+                    for (int k = 0; k < PA / 2; ++k)
+                        st.a[j][k] = (in && n + 2 * k < P.N ? (unsigned)e[2 * k] : 0u) | (in && n + 2 * k + 1 < P.N ? (unsigned)e[2 * k + 1] << 16 : 0u);
                 }
                 const uint8_t* q = P.q + r * P.ldq + (cin ? c : 0);
 #pragma unroll
-                for (int k = 0; k < PC / 4; ++k) st.q[j][k] = *reinterpret_cast<const unsigned*>(q + 4 * k);
-                st.s[j] = P.scale[r * P.CB + (cin ? c >> 5 : 0)];
-                if (!in) {
-#pragma unroll
-                    for (int k = 0; k < AD; ++k) st.a[j][k] = 0u;
-                }
-                if (!in || !cin) {
-#pragma unroll
-                    for (int k = 0; k < PC / 4; ++k) st.q[j][k] = 0u;
-                    st.s[j] = 0u;
+                for (int k = 0; k < PC / 4; ++k) {
+                    const unsigned w = *reinterpret_cast<const unsigned*>(q + 4 * k);
+                    st.q[j][k] = in && cin ? w : 0u;
                 }
             }
+            const int64_t row = m0 + step + sr;
+            const bool in = row < m1;
+            const uint8_t* sp = P.scale + (in ? row : m0) * P.CB;
+            const unsigned a = sp[sin ? sb : 0], b = PC == 8 ? sp[sin2 ? sb + 2 : 0] : 0u;
+            st.s = in && sin ? a : 0u;
+            if constexpr (PC == 8) st.s2 = in && sin2 ? b : 0u;
         }
     }
 };
@@ -177,15 +193,27 @@ __global__ __launch_bounds__(AW_THREADS, PA * PC <= 32 ? 2 : 1) void act8_wgrad_
 #pragma unroll
     for (int k = 0; k < PA; ++k) bias[k] = 0.f;
 
-    const AwLoader<DT, PA, PC, FAST> L(P, m0, m1, n0 + PA * i16, c0 + PC * i16, g);
+    const AwLoader<DT, PA, PC, FAST> L(P, m0, m1, n0 + PA * i16, c0 + PC * i16, g, c0, i16);
     auto compute = [&](AwStage<DT, PA, PC>& st) __attribute__((always_inline)) {
         // (rows and channels beyond the last: codes 0, scale byte 0 = 0.0)
         aw_bf16x8 xf[PC];
+        float sc[8];
+        const int blk = PC * i16 >> 5;                             // this lane's block of the tile
+        // (opaque here: combined where they are loaded, the two would be waited for there)
+        unsigned pair = st.s, high = PC == 8 ? st.s2 : 0u;
+        asm volatile("" : "+v"(pair));
+        asm volatile("" : "+v"(high));
+        pair |= high << 8;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const unsigned w = (unsigned)__shfl((int)pair, 16 * g + j + 8 * (blk & 1), 64);
+            sc[j] = act8_scale((w >> (8 * (blk >> 1))) & 255u);
+        }
 #pragma unroll
         for (int w = 0; w < PC / 2; ++w) {
             unsigned v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = aw_decode2<FMT>(st.q[j][w >> 1], act8_scale(st.s[j]), w & 1);
+            for (int j = 0; j < 8; ++j) v[j] = aw_decode2<FMT>(st.q[j][w >> 1], sc[j], w & 1);
 #pragma unroll
             for (int h = 0; h < 2; ++h)
                 xf[2 * w + h] = __builtin_bit_cast(aw_bf16x8, (act8_u32x4){aw_pair(v[0], v[1], h), aw_pair(v[2], v[3], h), aw_pair(v[4], v[5], h), aw_pair(v[6], v[7], h)});
@@ -358,29 +386,28 @@ __global__ __launch_bounds__(AW_THREADS) void act8_wgrad_join_kernel(const AwPar
     if (in) (isw ? P.dw : P.db)[isw ? i : i - nw] = (float)t;
 }
 
-// Tiles. bf16 in whole pieces: an edge of 128, or 64 where the weight is no wider (half the wasted products). fp16 / f32 (two or three
-// products per value, twice the raw registers) and rows read element by element: 64 x 64, two waves per SIMD. Waves: two tiles of dY
-// channels (else of X channels) side by side where there are two, so that a workgroup's partial tiles are joined in LDS only twice;
-// else all four waves split the rows of one tile.
-struct AwShape { int pa, pc, wn, wc, wk; };
+// Tiles, two waves per SIMD. bf16 in whole pieces: 64 x 128, or 64 x 64 where the weight is no wider (half the wasted products). fp16 /
+// f32 (two or three products per value, twice the raw registers) and rows read from any start: 64 x 64. (128 x 128, one wave per SIMD:
+// the same 86 us at 768 x 1536 over 25600 rows, a third fewer bytes through L1 but no second wave to fill the waits.) Waves: two tiles
+// of dY channels side by side where there are two, so that a workgroup's partial tiles are joined in LDS only twice; else all four
+// waves split the rows of one tile.
+struct AwShape { int pa, pc, wn, wk; };
 static AwShape aw_shape(int N, int C, bool wide) {
     AwShape s;
-    s.pa = !wide || N <= 64 ? 4 : 8;
+    s.pa = 4;
     s.pc = !wide || C <= 64 ? 4 : 8;
-    const int tn = (N + 16 * s.pa - 1) / (16 * s.pa), tc = (C + 16 * s.pc - 1) / (16 * s.pc);
-    s.wn = s.pa == 8 && s.pc == 8 && tn % 2 == 0 ? 2 : 1;
-    s.wc = s.pa == 8 && s.pc == 8 && s.wn == 1 && tc % 2 == 0 ? 2 : 1;
-    s.wk = 4 / (s.wn * s.wc);
+    const int tn = (N + 16 * s.pa - 1) / (16 * s.pa);
+    s.wn = s.pc == 8 && tn % 2 == 0 ? 2 : 1;
+    s.wk = 4 / s.wn;
     return s;
 }
 static void aw_geometry(AwParams& P, const AwShape& s, int64_t M, int N, int C) {
     P.M = M; P.N = N; P.C = C; P.CB = (C + 31) / 32;
     P.tiles_n = (N + 16 * s.pa * s.wn - 1) / (16 * s.pa * s.wn);
-    P.tiles_c = (C + 16 * s.pc * s.wc - 1) / (16 * s.pc * s.wc);
-    // ranges: as many workgroups as fit the CUs at once (two per CU below 128 x 128), at least 4 steps per wave, and less than
-    // 2 GiB of rows each
-    const int64_t tiles = (int64_t)P.tiles_n * P.tiles_c, steps = (M + AW_K - 1) / AW_K, most = (steps + 4 * s.wk - 1) / (4 * s.wk);
-    int64_t want = (s.pa * s.pc <= 32 ? 512 : 256) / tiles;
+    P.tiles_c = (C + 16 * s.pc - 1) / (16 * s.pc);
+    // ranges: as many workgroups as fit the CUs at once, at least a step per wave, and less than 2 GiB of rows each
+    const int64_t tiles = (int64_t)P.tiles_n * P.tiles_c, steps = (M + AW_K - 1) / AW_K, most = (steps + s.wk - 1) / s.wk;
+    int64_t want = 512 / tiles;
     if (want > most) want = most;
     if (want < 1) want = 1;
     int64_t per = (steps + want - 1) / want * AW_K;
@@ -423,10 +450,7 @@ template <int FMT> static int aw_dispatch(const AwParams& P, const AwShape& s, i
         if (dtype == H) return fast ? aw_launch<H, FMT, 4, 4, 1, 1, true>(P, st) : aw_launch<H, FMT, 4, 4, 1, 1, false>(P, st);
         return fast ? aw_launch<B, FMT, 4, 4, 1, 1, true>(P, st) : aw_launch<B, FMT, 4, 4, 1, 1, false>(P, st);
     }
-    if (s.pa == 4) return aw_launch<B, FMT, 4, 8, 1, 1, true>(P, st);
-    if (s.pc == 4) return aw_launch<B, FMT, 8, 4, 1, 1, true>(P, st);
-    if (s.wn == 2) return aw_launch<B, FMT, 8, 8, 2, 1, true>(P, st);
-    return s.wc == 2 ? aw_launch<B, FMT, 8, 8, 1, 2, true>(P, st) : aw_launch<B, FMT, 8, 8, 1, 1, true>(P, st);
+    return s.wn == 2 ? aw_launch<B, FMT, 4, 8, 2, 1, true>(P, st) : aw_launch<B, FMT, 4, 8, 1, 1, true>(P, st);
 }
 
 extern "C" int y5m_act8_wgrad(const void* dy, int64_t dy_batch_stride, int64_t dy_row_stride, int64_t N, int64_t S, int Cout, const void* q, int ldq,

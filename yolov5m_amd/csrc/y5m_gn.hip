@@ -1049,7 +1049,7 @@ static GnHeld gn_held(GnParams& P, bool blocks, const int* nrs) {
     if (P.N * P.slices >= (1ll << 31)) h.nr = 0;
     return h;
 }
-static const int GN_FWD_ROWS[] = {4, 12, 0}, GN_BWD_ROWS[2][3] = {{4, 12, 0}, {4, 0, 0}};       // (backward: 16 bits, f32)
+static const int GN_FWD_ROWS[] = {4, 16, 0}, GN_BWD_ROWS[2][3] = {{4, 12, 0}, {4, 0, 0}};       // (backward: 16 bits, f32)
 
 static int gn_check(int64_t N, int64_t S, int C, int G, int act, int dtype) {
     Y5M_REQUIRE(dtype == Y5M_F32 || dtype == Y5M_BF16 || dtype == Y5M_F16, "dtype");
@@ -1114,7 +1114,7 @@ template <int DT, int AL, int FMT> static int gn_fwd(GnParams& P, hipStream_t st
     if (h.nr == 0) return gn_fwd_split<DT, AL, FMT>(P, st);
     const int lds = (17 * h.threads + 4 * P.ct * 8) * (int)sizeof(float);
     if (h.nr == 4) GN_HELD_LAUNCH((gn_held_kernel<DT, AL, FMT, 4>), lds);
-    else GN_HELD_LAUNCH((gn_held_kernel<DT, AL, FMT, 12>), lds);
+    else GN_HELD_LAUNCH((gn_held_kernel<DT, AL, FMT, 16>), lds);
     Y5M_CHECK_LAUNCH("gn_held_kernel");
     return Y5M_OK;
 }
