@@ -47,6 +47,11 @@ _NOT_YET_ON_HARDWARE = {
 
 
 def pytest_collection_modifyitems(config, items):
+    # test_bf16_train_step_backward_variants_subprocess runs this suite's "per_layer_backward" tests in a child with the fused pointwise
+    # backward switched off (Y5M_BWD_PW=0). The full-size one asserts that the DEFAULT dispatch runs that kernel, so it is no test there.
+    if os.environ.get("Y5M_VARIANT_CHILD") == "1" and os.environ.get("Y5M_BWD_PW") == "0":
+        items[:] = [it for it in items if getattr(it, "originalname", it.name) != "test_bf16_per_layer_backward_full_size_default_dispatch"]
+
     def rank(it):
         if "test_gpu_zz_dp" in it.nodeid:
             return 2
