@@ -710,9 +710,6 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_apply_kernel(const GnParams
 // Slices of a sample follow each other on one XCD (the hardware deals workgroups round the 8 XCDs): a row's cache lines, which several
 // slices share, are fetched once.
 #define GN_HELD_THREADS 512
-#ifndef GN_HELD_MAX
-#define GN_HELD_MAX (8ll << 20)
-#endif
 
 struct GnSlice { int64_t n; int c0, nc, lr, lc, c, nv; bool in; };
 __device__ __forceinline__ GnSlice gn_slice(const GnParams& P) {
@@ -722,7 +719,7 @@ __device__ __forceinline__ GnSlice gn_slice(const GnParams& P) {
     w.n = b / (unsigned)P.slices;
     w.c0 = (int)(b - (unsigned)w.n * (unsigned)P.slices) * P.sc;
     w.nc = P.C - w.c0 < P.sc ? P.C - w.c0 : P.sc;
-    w.lr = (int)threadIdx.x / P.ct;
+    w.lr = gn_div((int)threadIdx.x, P.ctm);
     w.lc = (int)threadIdx.x - w.lr * P.ct;
     w.c = w.c0 + w.lc * 8;
     w.nv = w.c0 + w.nc - w.c;
@@ -761,11 +758,23 @@ template <int NS> __device__ __forceinline__ void gn_slice_sums(const GnParams& 
         __syncthreads();
     }
 }
-// f(group of the slice, sum over its channels of val(channel of the slice, i) in f64), one wave per group; f in lane 0
+// f(group of the slice, sums over its channels of val(channel of the slice, i) in f64): a thread per narrow group, a wave per wide one
 template <int NV, typename V, typename F> __device__ __forceinline__ void gn_slice_groups(const GnParams& P, const GnSlice& w, V val, F f) {
-    const int lane = threadIdx.x & 63, groups = w.nc / P.D;
+    const int groups = gn_div(w.nc, P.dm);
+    double a[NV];
+    if (P.D <= 32) {
+        for (int g = threadIdx.x; g < groups; g += (int)blockDim.x) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) a[i] = 0.0;
+            for (int d = 0; d < P.D; ++d)
+#pragma unroll
+                for (int i = 0; i < NV; ++i) a[i] += val(g * P.D + d, i);
+            f(g, a);
+        }
+        return;
+    }
+    const int lane = threadIdx.x & 63;
     for (int g = threadIdx.x >> 6; g < groups; g += (int)blockDim.x >> 6) {
-        double a[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i) a[i] = 0.0;
         for (int d = lane; d < P.D; d += 64)
@@ -808,7 +817,7 @@ __global__ __launch_bounds__(GN_HELD_THREADS) void gn_held_kernel(const GnParams
                        [&](int g, const double* s) __attribute__((always_inline)) { gm[g] = (float)(s[0] / K); });
     __syncthreads();
     const GnGroups gi = gn_groups(P, w.in ? w.lc * 8 : 0);         // (groups of the slice)
-    const int glast = w.nc / P.D - 1;
+    const int glast = gn_div(w.nc, P.dm) - 1;
 #pragma unroll
     for (int k = 0; k < 8; ++k) m[k] = gm[gi.g[k] < glast ? gi.g[k] : glast];
 #pragma unroll
@@ -833,7 +842,7 @@ __global__ __launch_bounds__(GN_HELD_THREADS) void gn_held_kernel(const GnParams
         const float mean = (float)((double)gm[g] + off), rs = (float)(1.0 / sqrt((var > 0.0 || var != var ? var : 0.0) + (double)P.eps));
         gm[g] = mean;
         gr[g] = rs;
-        const int64_t ng = w.n * P.G + w.c0 / P.D + g;
+        const int64_t ng = w.n * P.G + gn_div(w.c0, P.dm) + g;
         P.mean[ng] = mean;
         P.rstd[ng] = rs;
     });
@@ -905,12 +914,12 @@ __global__ __launch_bounds__(GN_HELD_THREADS) void gn_bwd_held_kernel(const GnPa
         graw[i] = load_raw8<DT, AL>(d + (int64_t)r * P.zr, at.nv);
     }
     const GnGroups gi = gn_groups(P, w.in ? w.lc * 8 : 0);
-    const int glast = w.nc / P.D - 1;
+    const int glast = gn_div(w.nc, P.dm) - 1;
     GnCoef k;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const int c = w.in && i < w.nv ? w.c + i : w.c0;
-        const int64_t ng = w.n * P.G + w.c0 / P.D + (gi.g[i] < glast ? gi.g[i] : glast);
+        const int64_t ng = w.n * P.G + gn_div(w.c0, P.dm) + (gi.g[i] < glast ? gi.g[i] : glast);
         k.mean[i] = P.mean[ng];
         k.rstd[i] = P.rstd[ng];
         k.gamma[i] = P.gamma ? P.gamma[c] : 1.0f;
@@ -1011,9 +1020,13 @@ static void gn_geometry(GnParams& P, bool quads, int rows, int arows) {
     P.ctm = gn_magic(P.ct);
 }
 
-// held: threads and rows per thread that hold a slice, NR = 0 where it does not fit. `nrs`: the row counts that are compiled, ascending
+// held: threads and rows per thread that hold a slice, NR = 0 where it does not fit or pays. `nrs`: the row counts that are compiled,
+// ascending; `most`: elements in all, above which the split form is faster -- except for samples of few rows, whose chunks would be
+// scraps. Held against split, 20 x 20 x 768 bf16 in 32 groups: forward of 1 / 16 / 32 / 64 images 9 / 14 / 17 / 30 us against 14 / 18 / 23 / 32,
+// of 256 165 against 105; backward of 1 / 8 / 16 / 32 images 13 / 14 / 23 / 39 against 21 / 24 / 29 / 36. 16384 x 768 tokens (one row
+// each): forward 92 against 940.
 struct GnHeld { int threads, nr; };
-static GnHeld gn_held(GnParams& P, bool blocks, const int* nrs) {
+static GnHeld gn_held(GnParams& P, bool blocks, const int* nrs, int64_t most) {
     int a = P.D, b = blocks ? 32 : 8;
     while (b) { const int t = a % b; a = b; b = t; }               // gcd
     const int64_t lcm = (int64_t)P.D / a * (blocks ? 32 : 8);
@@ -1023,7 +1036,7 @@ static GnHeld gn_held(GnParams& P, bool blocks, const int* nrs) {
         GnHeld h = {0, 0};
         const int sc = (int64_t)unit * k < P.C ? unit * k : P.C, ct = pieces(sc);
         for (int i = 0; nrs[i]; ++i)                               // (few rows a thread before few threads: what is serial is what counts)
-            for (int t = 256; t <= GN_HELD_THREADS; t *= 2) {
+            for (int t = 64; t <= GN_HELD_THREADS; t *= 2) {
                 if (ct > t || ceil_div(P.S, t / ct) > nrs[i]) continue;
                 h.threads = t;
                 h.nr = nrs[i];
@@ -1040,16 +1053,19 @@ static GnHeld gn_held(GnParams& P, bool blocks, const int* nrs) {
         h = w;
         ++k;
     }
-    if (h.nr == 0 || P.N * P.S * P.C > GN_HELD_MAX) return {0, 0};
+    if (h.nr == 0 || (P.N * P.S * P.C > most && P.S >= 128)) return {0, 0};
     P.sc = (int64_t)unit * k < P.C ? unit * k : P.C;
     P.slices = (int)ceil_div(P.C, P.sc);
     P.ct = pieces(P.sc);
     P.RP = h.threads / P.ct;
+    P.ctm = gn_magic(P.ct);
     P.CB = (P.C + 31) / 32;
     if (P.N * P.slices >= (1ll << 31)) h.nr = 0;
     return h;
 }
-static const int GN_FWD_ROWS[] = {4, 16, 0}, GN_BWD_ROWS[2][3] = {{4, 12, 0}, {4, 0, 0}};       // (backward: 16 bits, f32)
+static const int GN_FWD_ROWS[] = {4, 16, 0}, GN_BWD_ROWS[] = {4, 0};
+#define GN_HELD_FWD (24ll << 20)
+#define GN_HELD_BWD (6ll << 20)
 
 static int gn_check(int64_t N, int64_t S, int C, int G, int act, int dtype) {
     Y5M_REQUIRE(dtype == Y5M_F32 || dtype == Y5M_BF16 || dtype == Y5M_F16, "dtype");
@@ -1110,7 +1126,7 @@ template <int DT, int AL, int FMT> static int gn_fwd_split(GnParams& P, hipStrea
         hipLaunchKernelGGL(K, dim3((unsigned)(P.N * P.slices)), dim3(h.threads), lds, st, P);                                    \
     } while (0)
 template <int DT, int AL, int FMT> static int gn_fwd(GnParams& P, hipStream_t st) {
-    const GnHeld h = gn_held(P, FMT != Y5M_KEEP_NONE, GN_FWD_ROWS);
+    const GnHeld h = gn_held(P, FMT != Y5M_KEEP_NONE, GN_FWD_ROWS, GN_HELD_FWD);
     if (h.nr == 0) return gn_fwd_split<DT, AL, FMT>(P, st);
     const int lds = (17 * h.threads + 4 * P.ct * 8) * (int)sizeof(float);
     if (h.nr == 4) GN_HELD_LAUNCH((gn_held_kernel<DT, AL, FMT, 4>), lds);
@@ -1154,11 +1170,10 @@ extern "C" size_t y5m_gn_act_bwd_workspace_bytes(int64_t N, int64_t S, int C, in
 }
 
 template <int DT, int AL, int FMT> static int gn_bwd(GnParams& P, hipStream_t st) {
-    const GnHeld h = gn_held(P, false, GN_BWD_ROWS[DT == Y5M_F32]);
+    const GnHeld h = gn_held(P, false, GN_BWD_ROWS, GN_HELD_BWD);
     if (h.nr) {
         const int lds = (17 * h.threads + 4 * P.ct * 8) * (int)sizeof(float);
-        if (h.nr == 4) GN_HELD_LAUNCH((gn_bwd_held_kernel<DT, AL, FMT, 4>), lds);
-        else if constexpr (DT != Y5M_F32) GN_HELD_LAUNCH((gn_bwd_held_kernel<DT, AL, FMT, 12>), lds);
+        GN_HELD_LAUNCH((gn_bwd_held_kernel<DT, AL, FMT, 4>), lds);
         Y5M_CHECK_LAUNCH("gn_bwd_held_kernel");
     } else {
         gn_geometry(P, false, GN_ROWS, GN_APPLY_ROWS);
