@@ -10,7 +10,7 @@
 // (i = lane & 15, g = lane >> 4) loads rows 8 g .. 8 g + 7 of its OWN P channels (16 bytes of bf16, 8 of codes: a 16-lane group reads
 // 256 consecutive bytes of a row), and byte permutes (one per two values) turn the 8 x P block into P operands. Operand ja of lane i is
 // then channel P i + ja: the product of operands (ja, jb) is the 16 x 16 block of dW at rows P i + ja, columns P i' + jb, and the P x P
-// products of one 32-row step fill a (16 P)^2 tile: 128 x 128, 64 MFMAs, 256 accumulators a lane, one wave per SIMD, no barrier in the loop.
+// products of one 32-row step fill a (16 P)^2 tile (P = 8: 128 x 128, 64 MFMAs, 256 accumulators a lane), no barrier in the loop.
 // A lane ends up with P consecutive columns of a row of dW: 16-byte stores.
 // The four waves of a workgroup are WN x WC tiles side by side (they share operands through L1) times WK interleaved parts of the
 // rows, added in LDS; row ranges of different workgroups are joined from f32 partial tiles by a second launch in a fixed order (no
@@ -386,28 +386,29 @@ __global__ __launch_bounds__(AW_THREADS) void act8_wgrad_join_kernel(const AwPar
     if (in) (isw ? P.dw : P.db)[isw ? i : i - nw] = (float)t;
 }
 
-// Tiles, two waves per SIMD. bf16 in whole pieces: 64 x 128, or 64 x 64 where the weight is no wider (half the wasted products). fp16 /
-// f32 (two or three products per value, twice the raw registers) and rows read from any start: 64 x 64. (128 x 128, one wave per SIMD:
-// the same 86 us at 768 x 1536 over 25600 rows, a third fewer bytes through L1 but no second wave to fill the waits.) Waves: two tiles
-// of dY channels side by side where there are two, so that a workgroup's partial tiles are joined in LDS only twice; else all four
-// waves split the rows of one tile.
-struct AwShape { int pa, pc, wn, wk; };
+// Tiles. bf16 in whole pieces: 128 x 128 at one wave per SIMD; 64 x 128 / 64 x 64 at two where the weight is no wider (half the wasted
+// products). (64 x 128 for all: 120 us instead of 112 for store + gradient at 768 x 1536 over 25600 rows; the second wave fills the
+// waits, but every byte goes through L1 half as often again.) fp16 / f32 (two or three products per value, twice the raw registers) and
+// rows read from any start: 64 x 64. Waves: two tiles of dY channels (else of X channels) side by side where there are two, so that a
+// workgroup's partial tiles are joined in LDS only twice; else all four waves split the rows of one tile.
+struct AwShape { int pa, pc, wn, wc, wk; };
 static AwShape aw_shape(int N, int C, bool wide) {
     AwShape s;
-    s.pa = 4;
     s.pc = !wide || C <= 64 ? 4 : 8;
-    const int tn = (N + 16 * s.pa - 1) / (16 * s.pa);
-    s.wn = s.pc == 8 && tn % 2 == 0 ? 2 : 1;
-    s.wk = 4 / s.wn;
+    s.pa = s.pc == 4 || N <= 64 ? 4 : 8;
+    const int tn = (N + 16 * s.pa - 1) / (16 * s.pa), tc = (C + 16 * s.pc - 1) / (16 * s.pc);
+    s.wn = s.pa == 8 && tn % 2 == 0 ? 2 : 1;
+    s.wc = s.pa == 8 && s.wn == 1 && tc % 2 == 0 ? 2 : 1;
+    s.wk = 4 / (s.wn * s.wc);
     return s;
 }
 static void aw_geometry(AwParams& P, const AwShape& s, int64_t M, int N, int C) {
     P.M = M; P.N = N; P.C = C; P.CB = (C + 31) / 32;
     P.tiles_n = (N + 16 * s.pa * s.wn - 1) / (16 * s.pa * s.wn);
-    P.tiles_c = (C + 16 * s.pc - 1) / (16 * s.pc);
+    P.tiles_c = (C + 16 * s.pc * s.wc - 1) / (16 * s.pc * s.wc);
     // ranges: as many workgroups as fit the CUs at once, at least a step per wave, and less than 2 GiB of rows each
     const int64_t tiles = (int64_t)P.tiles_n * P.tiles_c, steps = (M + AW_K - 1) / AW_K, most = (steps + s.wk - 1) / s.wk;
-    int64_t want = 512 / tiles;
+    int64_t want = (s.pa == 8 ? 256 : 512) / tiles;
     if (want > most) want = most;
     if (want < 1) want = 1;
     int64_t per = (steps + want - 1) / want * AW_K;
@@ -450,7 +451,9 @@ template <int FMT> static int aw_dispatch(const AwParams& P, const AwShape& s, i
         if (dtype == H) return fast ? aw_launch<H, FMT, 4, 4, 1, 1, true>(P, st) : aw_launch<H, FMT, 4, 4, 1, 1, false>(P, st);
         return fast ? aw_launch<B, FMT, 4, 4, 1, 1, true>(P, st) : aw_launch<B, FMT, 4, 4, 1, 1, false>(P, st);
     }
-    return s.wn == 2 ? aw_launch<B, FMT, 4, 8, 2, 1, true>(P, st) : aw_launch<B, FMT, 4, 8, 1, 1, true>(P, st);
+    if (s.pa == 4) return aw_launch<B, FMT, 4, 8, 1, 1, true>(P, st);
+    if (s.wn == 2) return aw_launch<B, FMT, 8, 8, 2, 1, true>(P, st);
+    return s.wc == 2 ? aw_launch<B, FMT, 8, 8, 1, 2, true>(P, st) : aw_launch<B, FMT, 8, 8, 1, 1, true>(P, st);
 }
 
 extern "C" int y5m_act8_wgrad(const void* dy, int64_t dy_batch_stride, int64_t dy_row_stride, int64_t N, int64_t S, int Cout, const void* q, int ldq,
