@@ -36,6 +36,7 @@ struct GnParams {
     int64_t N, xn, xr, zn, zr, on, orow;
     int S, C, G, D, ldq, CB, act;
     float eps;
+    double inv_k;                            // 1 / (S D)
     int CV, ct, tiles, RP, chunks, rpc;      // split: pieces per row / per column tile, column tiles, rows side by side, row chunks, rows per chunk
     int achunks, arpc;                       // the apply pass's chunks
     unsigned ctm, dm;                        // ceil(2^32 / ct), ceil(2^32 / D): quotients of threads and channels by one multiply
@@ -273,12 +274,12 @@ __global__ __launch_bounds__(GN_THREADS) void gn_stats_join_kernel(const GnParam
         }
     gn_block_sum<3>(v, red);
     if (threadIdx.x == 0) {
-        const double K = (double)P.S * (double)P.D, off = v[0] / K;
-        double var = v[2] / K + v[1] / K - off * off;
+        const double off = v[0] * P.inv_k;
+        double var = (v[2] + v[1]) * P.inv_k - off * off;
         if (!(var > 0.0) && var == var) var = 0.0;                 // (a NaN stays)
         const int64_t ng = b * P.G + g;
         P.mean[ng] = (float)(ref + off);
-        P.rstd[ng] = (float)(1.0 / sqrt(var + (double)P.eps));
+        P.rstd[ng] = 1.0f / sqrtf((float)(var + (double)P.eps));
     }
 }
 
@@ -600,10 +601,7 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_join_kernel(const GnParams 
     }
     gn_block_sum<2>(v, red);
     if (threadIdx.x == 0) {
-        const double K = (double)P.S * (double)P.D;
-        float* ab = P.ab + (n * P.G + g) * 2;
-        ab[0] = (float)(v[0] / K);
-        ab[1] = (float)(v[1] / K);
+        *reinterpret_cast<float2*>(P.ab + (n * P.G + g) * 2) = make_float2((float)(v[0] * P.inv_k), (float)(v[1] * P.inv_k));
     }
 }
 
@@ -800,7 +798,6 @@ __global__ __launch_bounds__(GN_HELD_THREADS) void gn_held_kernel(const GnParams
         const int r = lr + i * P.RP;
         raw[i] = load_raw8<DT, AL>(b + (int64_t)(r < P.S ? r : P.S - 1) * P.xr, nvl);
     }
-    const double K = (double)P.S * (double)P.D;
     float a[16], m[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) a[k] = 0.f;
@@ -814,7 +811,7 @@ __global__ __launch_bounds__(GN_HELD_THREADS) void gn_held_kernel(const GnParams
     }
     gn_slice_sums<1>(P, w, a, red, sub, tot);
     gn_slice_groups<1>(P, w, [&](int c, int) __attribute__((always_inline)) { return (double)tot[c]; },
-                       [&](int g, const double* s) __attribute__((always_inline)) { gm[g] = (float)(s[0] / K); });
+                       [&](int g, const double* s) __attribute__((always_inline)) { gm[g] = (float)(s[0] * P.inv_k); });
     __syncthreads();
     const GnGroups gi = gn_groups(P, w.in ? w.lc * 8 : 0);         // (groups of the slice)
     const int glast = gn_div(w.nc, P.dm) - 1;
@@ -838,8 +835,8 @@ __global__ __launch_bounds__(GN_HELD_THREADS) void gn_held_kernel(const GnParams
     gn_slice_sums<2>(P, w, a, red, sub, tot);
     const int wd = P.ct * 8;
     gn_slice_groups<2>(P, w, [&](int c, int i) __attribute__((always_inline)) { return (double)tot[i * wd + c]; }, [&](int g, const double* s) __attribute__((always_inline)) {
-        const double off = s[0] / K, var = s[1] / K - off * off;
-        const float mean = (float)((double)gm[g] + off), rs = (float)(1.0 / sqrt((var > 0.0 || var != var ? var : 0.0) + (double)P.eps));
+        const double off = s[0] * P.inv_k, var = s[1] * P.inv_k - off * off;
+        const float mean = (float)((double)gm[g] + off), rs = 1.0f / sqrtf((float)((var > 0.0 || var != var ? var : 0.0) + (double)P.eps));
         gm[g] = mean;
         gr[g] = rs;
         const int64_t ng = w.n * P.G + gn_div(w.c0, P.dm) + g;
@@ -964,10 +961,9 @@ __global__ __launch_bounds__(GN_HELD_THREADS) void gn_bwd_held_kernel(const GnPa
         }
     }
     __syncthreads();
-    const double K = (double)P.S * (double)P.D;
     gn_slice_groups<2>(P, w, [&](int c, int i) __attribute__((always_inline)) { return (double)tot[i * wd + c]; }, [&](int g, const double* s) __attribute__((always_inline)) {
-        gA[g] = (float)(s[0] / K);
-        gB[g] = (float)(s[1] / K);
+        gA[g] = (float)(s[0] * P.inv_k);
+        gB[g] = (float)(s[1] * P.inv_k);
     });
     __syncthreads();
     // dx = r gamma dt - r A - r B xhat = c1 dt + (c2 xhat + c3)
@@ -1026,10 +1022,12 @@ static void gn_geometry(GnParams& P, bool quads, int rows, int arows) {
 // of 256 165 against 105; backward of 1 / 8 / 16 / 32 images 13 / 14 / 23 / 39 against 21 / 24 / 29 / 36. 16384 x 768 tokens (one row
 // each): forward 92 against 940.
 struct GnHeld { int threads, nr; };
-static GnHeld gn_held(GnParams& P, bool blocks, const int* nrs, int64_t most) {
-    int a = P.D, b = blocks ? 32 : 8;
+static GnHeld gn_held(GnParams& P, bool blocks, bool aligned, const int* nrs, int64_t most) {
+    // whole groups, whole blocks or pieces; rows that start anywhere may be cut anywhere (at 8 channels or more: load_raw8)
+    const int cut = blocks ? 32 : 8;
+    int a = P.D, b = cut;
     while (b) { const int t = a % b; a = b; b = t; }               // gcd
-    const int64_t lcm = (int64_t)P.D / a * (blocks ? 32 : 8);
+    const int64_t lcm = blocks || aligned ? (int64_t)P.D / a * cut : ceil_div(8, P.D) * P.D;
     const int unit = lcm < P.C ? (int)lcm : P.C, units = (int)ceil_div(P.C, unit);
     auto pieces = [&](int sc) { const int p = (sc + 7) / 8; return blocks ? (p + 3) / 4 * 4 : p; };
     auto fit = [&](int k) {
@@ -1076,6 +1074,7 @@ static int gn_check(int64_t N, int64_t S, int C, int G, int act, int dtype) {
 }
 static void gn_sizes(GnParams& P, int64_t N, int64_t S, int C, int G) {
     P.N = N; P.S = (int)S; P.C = C; P.G = G; P.D = C / G; P.dm = gn_magic(P.D);
+    P.inv_k = 1.0 / ((double)S * (double)P.D);
 }
 
 extern "C" size_t y5m_gn_act_workspace_bytes(int64_t N, int64_t S, int C, int G) {
@@ -1126,7 +1125,7 @@ template <int DT, int AL, int FMT> static int gn_fwd_split(GnParams& P, hipStrea
         hipLaunchKernelGGL(K, dim3((unsigned)(P.N * P.slices)), dim3(h.threads), lds, st, P);                                    \
     } while (0)
 template <int DT, int AL, int FMT> static int gn_fwd(GnParams& P, hipStream_t st) {
-    const GnHeld h = gn_held(P, FMT != Y5M_KEEP_NONE, GN_FWD_ROWS, GN_HELD_FWD);
+    const GnHeld h = gn_held(P, FMT != Y5M_KEEP_NONE, AL > 0, GN_FWD_ROWS, GN_HELD_FWD);
     if (h.nr == 0) return gn_fwd_split<DT, AL, FMT>(P, st);
     const int lds = (17 * h.threads + 4 * P.ct * 8) * (int)sizeof(float);
     if (h.nr == 4) GN_HELD_LAUNCH((gn_held_kernel<DT, AL, FMT, 4>), lds);
@@ -1170,7 +1169,7 @@ extern "C" size_t y5m_gn_act_bwd_workspace_bytes(int64_t N, int64_t S, int C, in
 }
 
 template <int DT, int AL, int FMT> static int gn_bwd(GnParams& P, hipStream_t st) {
-    const GnHeld h = gn_held(P, false, GN_BWD_ROWS, GN_HELD_BWD);
+    const GnHeld h = gn_held(P, false, AL > 0 || FMT != Y5M_KEEP_NONE, GN_BWD_ROWS, GN_HELD_BWD);
     if (h.nr) {
         const int lds = (17 * h.threads + 4 * P.ct * 8) * (int)sizeof(float);
         GN_HELD_LAUNCH((gn_bwd_held_kernel<DT, AL, FMT, 4>), lds);
