@@ -10,6 +10,7 @@
 // exponent): the largest values round to a code that stays finite when read back. A block holding a NaN or an infinity gets scale
 // byte 255 and reads back as NaN throughout: an overflow in a training step must reach the gradients, and int8 has no NaN code.
 #pragma once
+#include <atomic>
 #include "y5m_common.h"
 
 typedef _Float16 y5m_f16;
@@ -204,4 +205,19 @@ static inline int rows_mode(bool aligned, int C) { return aligned ? 1 : C >= 8 ?
 static inline bool rows_aligned16(const void* p, int64_t sn, int64_t sr, int64_t N, int64_t S, int C, int dtype) {
     const int per = dtype == Y5M_F32 ? 4 : 8;
     return ((uintptr_t)p & 15) == 0 && C % 8 == 0 && (S <= 1 || sr % per == 0) && (N <= 1 || sn % per == 0);
+}
+// host: dynamic LDS above 64 KB has to be asked for, per kernel and device; `asked`: one bit for each of the first 64 devices
+static inline bool lds_ask(const void* kernel, int need, int most, std::atomic<uint64_t>& asked) {
+    if (need <= 64 * 1024) return true;
+    int dev = 64;
+    (void)hipGetDevice(&dev);
+    const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
+    if (asked.load(std::memory_order_relaxed) & bit) return true;
+    if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, most) != hipSuccess) {
+        (void)hipGetLastError();
+        y5m_set_error("%d bytes of LDS refused", most);
+        return false;
+    }
+    asked.fetch_or(bit, std::memory_order_relaxed);
+    return true;
 }

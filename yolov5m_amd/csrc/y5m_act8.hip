@@ -111,7 +111,7 @@ static void act8_geometry(Act8Params& P) {
     P.RP = A8_THREADS / P.ct;
     // 8 rows a thread; more where the grid would not fit
     int64_t rpc = (int64_t)P.RP * 8;
-    while ((P.M + rpc - 1) / rpc * P.tiles >= (1ll << 31)) rpc *= 2;
+    while ((P.M + rpc - 1) / rpc * P.tiles >= (1ll << 24)) rpc *= 2;
     P.rpc = (int)rpc;
 }
 
@@ -130,7 +130,7 @@ static void act8_geometry(Act8Params& P) {
 #define ACT8_D3(KERN, DT, FMT, NT)                                                                                                \
     do {                                                                                                                          \
         if (al < 0) ACT8_GO((KERN<DT, FMT, -1>));                                                                                 \
-        else if (al == 0) ACT8_GO((KERN<DT, FMT, 0>));                                                                                     \
+        else if (al == 0) ACT8_GO((KERN<DT, FMT, 0>));                                                                            \
         else if (nt) ACT8_GO((KERN<DT, FMT, NT>));                                                                                \
         else ACT8_GO((KERN<DT, FMT, 1>));                                                                                         \
     } while (0)

@@ -432,11 +432,8 @@ template <int DT, int FMT, int PA, int PC, int WN, int WC, bool FAST, bool DB>
 static int aw_launch_db(const AwParams& P, hipStream_t st) {
     constexpr int WK = 4 / (WN * WC), lds = ((WK - 1) * WN * WC * (PA / 2 * PC * 4) * 64 + WK * WN * 16 * PA) * (int)sizeof(float);
     static_assert(lds <= 160 * 1024, "LDS");
-    if constexpr (lds > 64 * 1024) {
-        static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(act8_wgrad_kernel<DT, FMT, PA, PC, WN, WC, WK, FAST, DB>),
-                                                        hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-        if (e != hipSuccess) { y5m_set_error("act8_wgrad_kernel: %d bytes of LDS refused", lds); return Y5M_ELAUNCH; }
-    }
+    static std::atomic<uint64_t> asked{0};
+    if (!lds_ask(reinterpret_cast<const void*>(act8_wgrad_kernel<DT, FMT, PA, PC, WN, WC, WK, FAST, DB>), lds, lds, asked)) return Y5M_ELAUNCH;
     hipLaunchKernelGGL((act8_wgrad_kernel<DT, FMT, PA, PC, WN, WC, WK, FAST, DB>), dim3((unsigned)((int64_t)P.tiles_n * P.tiles_c * P.ranges)), dim3(AW_THREADS), lds, st, P);
     Y5M_CHECK_LAUNCH("act8_wgrad_kernel");
     return Y5M_OK;
@@ -487,7 +484,7 @@ extern "C" int y5m_act8_wgrad(const void* dy, int64_t dy_batch_stride, int64_t d
     P.part = static_cast<float*>(ws);
     P.dbpart = db ? P.part + (size_t)P.ranges * Cout * C : nullptr;
     P.dw = dw; P.db = db;
-    Y5M_REQUIRE((int64_t)P.tiles_n * P.tiles_c * P.ranges < (1ll << 31), "too many workgroups");
+    Y5M_REQUIRE((int64_t)P.tiles_n * P.tiles_c * P.ranges < (1ll << 24) && (int64_t)Cout * C * P.slots < (1ll << 31), "too many workgroups");
     const int rc = fmt == Y5M_KEEP_E4M3 ? aw_dispatch<Y5M_KEEP_E4M3>(P, s, dtype, fast, y5m_stream(stream)) : aw_dispatch<Y5M_KEEP_INT8>(P, s, dtype, fast, y5m_stream(stream));
     if (rc != Y5M_OK) return rc;
     const int64_t items = (int64_t)Cout * C + (db ? Cout : 0), per = AW_THREADS / P.slots;

@@ -248,8 +248,9 @@ __device__ __forceinline__ GnWalk gn_walk(int D) {
 
 __global__ __launch_bounds__(GN_THREADS) void gn_stats_join_kernel(const GnParams P) {
     __shared__ double red[12];
-    const int64_t b = blockIdx.x / (unsigned)P.G;
-    const int g = (int)(blockIdx.x - b * P.G);
+    const int64_t b = (int64_t)blockIdx.z * gridDim.y + blockIdx.y;
+    const int g = (int)blockIdx.x;
+    if (b >= P.N) return;
     const float* part = P.part + (size_t)b * P.chunks * 2 * P.C + 2 * g * P.D;
     const GnWalk k = gn_walk(P.D);
     const double ref = (double)part[0];
@@ -559,9 +560,10 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_reduce_kernel(const GnParam
 // channel sums of a sample and A, B of its groups, one workgroup per (sample, group)
 __global__ __launch_bounds__(GN_THREADS) void gn_bwd_join_kernel(const GnParams P) {
     __shared__ double red[2 * GN_THREADS];
-    const int64_t b = blockIdx.x / (unsigned)P.G, n = b;
-    const int g = (int)(blockIdx.x - b * P.G);
-    const float* part = P.part + (size_t)b * P.chunks * 2 * P.C + 2 * g * P.D;
+    const int64_t n = (int64_t)blockIdx.z * gridDim.y + blockIdx.y;
+    const int g = (int)blockIdx.x;
+    if (n >= P.N) return;
+    const float* part = P.part + (size_t)n * P.chunks * 2 * P.C + 2 * g * P.D;
     const GnWalk k = gn_walk(P.D);
     double v[2] = {0.0, 0.0};
     for (int d0 = 0; d0 < P.D; d0 += GN_THREADS) {                 // (uniform: every thread meets at the barriers)
@@ -1052,13 +1054,13 @@ static GnHeld gn_held(GnParams& P, bool blocks, bool aligned, const int* nrs, in
         ++k;
     }
     if (h.nr == 0 || (P.N * P.S * P.C > most && P.S >= 128)) return {0, 0};
+    if (P.N * ceil_div(units, k) * h.threads >= (1ll << 32)) return {0, 0};          // (the launch's threads are counted in 32 bits)
     P.sc = (int64_t)unit * k < P.C ? unit * k : P.C;
     P.slices = (int)ceil_div(P.C, P.sc);
     P.ct = pieces(P.sc);
     P.RP = h.threads / P.ct;
     P.ctm = gn_magic(P.ct);
     P.CB = (P.C + 31) / 32;
-    if (P.N * P.slices >= (1ll << 31)) h.nr = 0;
     return h;
 }
 static const int GN_FWD_ROWS[] = {4, 16, 0}, GN_BWD_ROWS[] = {4, 0};
@@ -1100,28 +1102,26 @@ static dim3 gn_grid(int64_t x, int64_t N) {
     const int64_t y = N < 32768 ? N : 32768;
     return dim3((unsigned)x, (unsigned)y, (unsigned)ceil_div(N, y));
 }
-#define GN_LAUNCH2(K, x) hipLaunchKernelGGL(K, gn_grid((int64_t)(x) * P.tiles, P.N), dim3(GN_THREADS), 0, st, P)
-#define GN_LIMITS Y5M_REQUIRE((int64_t)P.achunks * P.tiles + P.C < (1ll << 31) && (int64_t)P.chunks * P.tiles < (1ll << 31) && P.N * P.G < (1ll << 31), "too many workgroups")
+// (at most 65536 chunks of 32 tiles, or 65535 groups: every dimension is below 2^24 workgroups = 2^32 threads)
+#define GN_LAUNCH2(K, x) hipLaunchKernelGGL(K, gn_grid((int64_t)(x), P.N), dim3(GN_THREADS), 0, st, P)
 
 template <int DT, int AL, int FMT> static int gn_fwd_split(GnParams& P, hipStream_t st) {
     gn_geometry(P, FMT != Y5M_KEEP_NONE, GN_ROWS, GN_APPLY_ROWS);
-    GN_LIMITS;
-    GN_LAUNCH2((gn_stats_kernel<DT, AL>), P.chunks);
-    GN_LAUNCH(gn_stats_join_kernel, P.N * P.G);
+    GN_LAUNCH2((gn_stats_kernel<DT, AL>), P.chunks * P.tiles);
+    GN_LAUNCH2(gn_stats_join_kernel, P.G);
     if constexpr (AL > 0) {
-        if (rows_past_caches(P.N * P.S, P.C, DT)) GN_LAUNCH2((gn_apply_kernel<DT, 2, FMT>), P.achunks);
-        else GN_LAUNCH2((gn_apply_kernel<DT, 1, FMT>), P.achunks);
+        if (rows_past_caches(P.N * P.S, P.C, DT)) GN_LAUNCH2((gn_apply_kernel<DT, 2, FMT>), P.achunks * P.tiles);
+        else GN_LAUNCH2((gn_apply_kernel<DT, 1, FMT>), P.achunks * P.tiles);
     } else {
-        GN_LAUNCH2((gn_apply_kernel<DT, AL, FMT>), P.achunks);
+        GN_LAUNCH2((gn_apply_kernel<DT, AL, FMT>), P.achunks * P.tiles);
     }
     Y5M_CHECK_LAUNCH("gn_apply_kernel");
     return Y5M_OK;
 }
-// LDS above 64 KB has to be asked for, once per kernel
 #define GN_HELD_LAUNCH(K, lds)                                                                                                   \
     do {                                                                                                                         \
-        static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(K), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024); \
-        if (e != hipSuccess) { y5m_set_error("%s: LDS refused", #K); return Y5M_ELAUNCH; }                                       \
+        static std::atomic<uint64_t> asked{0};                                                                                   \
+        if (!lds_ask(reinterpret_cast<const void*>(K), lds, 160 * 1024, asked)) return Y5M_ELAUNCH;                              \
         hipLaunchKernelGGL(K, dim3((unsigned)(P.N * P.slices)), dim3(h.threads), lds, st, P);                                    \
     } while (0)
 template <int DT, int AL, int FMT> static int gn_fwd(GnParams& P, hipStream_t st) {
@@ -1176,14 +1176,13 @@ template <int DT, int AL, int FMT> static int gn_bwd(GnParams& P, hipStream_t st
         Y5M_CHECK_LAUNCH("gn_bwd_held_kernel");
     } else {
         gn_geometry(P, false, GN_ROWS, GN_APPLY_ROWS);
-            GN_LIMITS;
-        GN_LAUNCH2((gn_bwd_reduce_kernel<DT, AL, FMT>), P.chunks);
-        GN_LAUNCH(gn_bwd_join_kernel, P.N * P.G);
+                GN_LAUNCH2((gn_bwd_reduce_kernel<DT, AL, FMT>), P.chunks * P.tiles);
+        GN_LAUNCH2(gn_bwd_join_kernel, P.G);
         if constexpr (AL > 0) {
-            if (rows_past_caches(P.N * P.S, P.C, DT)) GN_LAUNCH2((gn_bwd_apply_kernel<DT, 2, FMT>), P.achunks);
-            else GN_LAUNCH2((gn_bwd_apply_kernel<DT, 1, FMT>), P.achunks);
+            if (rows_past_caches(P.N * P.S, P.C, DT)) GN_LAUNCH2((gn_bwd_apply_kernel<DT, 2, FMT>), P.achunks * P.tiles);
+            else GN_LAUNCH2((gn_bwd_apply_kernel<DT, 1, FMT>), P.achunks * P.tiles);
         } else {
-            GN_LAUNCH2((gn_bwd_apply_kernel<DT, AL, FMT>), P.achunks);
+            GN_LAUNCH2((gn_bwd_apply_kernel<DT, AL, FMT>), P.achunks * P.tiles);
         }
         Y5M_CHECK_LAUNCH("gn_bwd_apply_kernel");
     }
