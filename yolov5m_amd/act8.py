@@ -13,6 +13,7 @@ The rows of a tensor are its positions (n, *spatial), each C consecutive values:
 as x.transpose(1, 2), and channel slices of wider buffers. A tensor laid out otherwise is refused, not copied.
 """
 import contextlib
+import math
 
 import torch
 
@@ -55,6 +56,8 @@ def rows_of(t, name):
     n, c = shape[0], shape[1]
     if c == 0:
         raise Y5MError(f"{name}: no channels")
+    if t.numel() == 0:                                               # (strides mean nothing)
+        return n, math.prod(shape[2:]), c, 0, c
     s, row, pitch = 1, None, 0
     for d in range(len(shape) - 1, 1, -1):
         size = shape[d]
@@ -67,7 +70,7 @@ def rows_of(t, name):
             raise Y5MError(f"{name}: the positions must lie at one distance from each other (channels last); strides {tuple(st)} of "
                            f"shape {tuple(shape)}: use .contiguous(memory_format=torch.channels_last)")
         pitch = st[d] * size
-    if c > 1 and st[1] != 1 and n * s > 0:
+    if c > 1 and st[1] != 1:
         raise Y5MError(f"{name}: channels must be the dense dimension (channels last); strides {tuple(st)} of shape {tuple(shape)}: "
                        "use .contiguous(memory_format=torch.channels_last)")
     return n, s, c, st[0], (c if row is None else row)
