@@ -35,6 +35,8 @@ class CBL(nn.Module):
         conv = nn.Conv2d(in_channels, out_channels, kernel_size, stride, padding, bias=False)
         self.norm_groups = norm_groups
         if norm_groups is None:
+            if keep != "x":
+                raise _lib.Y5MError(f"keep {keep!r} needs norm_groups")
             bn = nn.BatchNorm2d(out_channels, eps=1e-3, momentum=0.03)
         else:
             from .group_norm import GroupNormAct
