@@ -236,3 +236,64 @@ def test_c_entry_refuses_what_it_cannot_run():
     torch.cuda.synchronize()
     assert (q == 7).all() and (s == 7).all() and (dw == 3.0).all()
     assert isinstance(ctypes.c_size_t(need).value, int)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "fp16"])
+def test_one_row_per_image_and_rows_apart(dtype):
+    """(N, C) matrices cut out of wider ones, batches that do not follow each other at the rows' distance: stored form and gradient"""
+    from yolov5m_amd.act8 import act8_load, act8_store, act8_wgrad
+    flat = torch.randn(70, 256, generator=_gen(11)).to(DT[dtype]).to(DEV)
+    maps = rows_tensor((3, 160, 9, 8), dtype, 12)
+    for x, dy in ((flat[:, 8:72], flat[:, 128:168]), (flat[:, 3:72], flat[:, 101:150]), (maps[:, :72, 1:8], maps[:, 72:136, 1:8]), (maps[::2, 5:60], maps[::2, 64:160])):
+        kept = act8_store(x, "int8")
+        assert same(act8_load(kept).cpu().movedim(1, -1).double(), stored_values(x, "int8")[0].to(DT[dtype]).double())
+        dw, db = act8_wgrad(dy, kept, bias=True)
+        xv = stored_values(x, "int8")[0].reshape(-1, x.shape[1])
+        dv = dy.cpu().double().movedim(1, -1).reshape(-1, dy.shape[1])
+        assert ((dw.cpu().double() - dv.t() @ xv).abs() <= 96 * U * (dv.abs().t() @ xv.abs())).all()
+        assert ((db.cpu().double() - dv.sum(0)).abs() <= 160 * U * dv.abs().sum(0)).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "fp16"])
+@pytest.mark.parametrize("shape", [(1, 100, 5, 5), (1, 160, 40)])
+def test_wgrad_nan_in_any_block(shape, dtype):
+    """e4m3: a block that is not finite reaches its own columns only, the last (short) block as well; a NaN of dy its own rows only"""
+    from yolov5m_amd.act8 import act8_store, act8_wgrad
+    c = shape[1]
+    for ch in (2, 70, c - 1):
+        x, dy = rows_tensor(shape, "bf16", 13), rows_tensor((1, 72, *shape[2:]), dtype, 14)
+        x[(0, ch) + (2,) * (len(shape) - 2)] = float("nan")
+        dw, _ = act8_wgrad(dy, act8_store(x, "e4m3"))
+        bad = torch.zeros(c, dtype=torch.bool, device=DEV)
+        bad[ch // 32 * 32:ch // 32 * 32 + 32] = True
+        assert torch.isnan(dw[:, bad]).all() and torch.isfinite(dw[:, ~bad]).all()
+    x = rows_tensor(shape, "bf16", 13)
+    dy[(0, 37) + (1,) * (len(shape) - 2)] = float("nan")
+    dw, db = act8_wgrad(dy, act8_store(x, "e4m3"), bias=True)
+    rows = torch.arange(72, device=DEV) == 37
+    assert torch.isnan(dw[rows]).all() and torch.isfinite(dw[~rows]).all() and torch.isnan(db[rows]).all() and torch.isfinite(db[~rows]).all()
+
+
+def test_large_tensors_read_back():
+    """more than 64 MB: stored past the caches, by kernels of their own"""
+    if DEV != "cuda":
+        pytest.skip("36 million elements")
+    from yolov5m_amd.act8 import act8_load, act8_store
+    x = rows_tensor((2, 72, 500, 501), "bf16", 15)
+    for fmt in ("e4m3", "int8"):
+        assert same(act8_load(act8_store(x, fmt)).cpu().movedim(1, -1).double(), stored_values(x, fmt)[0])
+
+
+def test_wgrad_rows_far_apart():
+    """rows of dy at a distance that one range's 32-bit offsets cannot hold"""
+    if DEV != "cuda":
+        pytest.skip("6 GB")
+    from yolov5m_amd.act8 import act8_load, act8_store, act8_wgrad
+    wide = torch.empty((3000, 1 << 20), dtype=torch.bfloat16, device=DEV)
+    dy = wide[:, 1 << 19:(1 << 19) + 160].t()[None]
+    dy.copy_(rows_tensor((1, 160, 3000), "bf16", 16))
+    kept = act8_store(rows_tensor((1, 200, 3000), "bf16", 17), "e4m3")
+    dw, db = act8_wgrad(dy, kept, bias=True)
+    xv, dv = act8_load(kept).cpu().double()[0].t(), dy.cpu().double()[0].t()
+    assert ((dw.cpu().double() - dv.t() @ xv).abs() <= 96 * U * (dv.abs().t() @ xv.abs())).all()
+    assert ((db.cpu().double() - dv.sum(0)).abs() <= 160 * U * dv.abs().sum(0)).all()

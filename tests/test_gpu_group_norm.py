@@ -435,3 +435,144 @@ def test_c3_block_trains_with_group_norm_and_kept_activations():
     want = cbl(m.c_out, torch.cat([a, cbl(m.c_skipped, xd)], 1))
     got = m(x).detach().cpu().double()
     assert (got - want).abs().max() <= 2e-4 * want.abs().max()
+
+
+@pytest.mark.parametrize("keep", ["x", "int8"])
+@pytest.mark.parametrize("case", [((3, 8200), 1), ((3, 8200), 8), ((300, 24), 3), ((2, 40, 3), 40)])
+def test_samples_of_few_rows(case, keep):
+    """one row per sample (tokens, class logits), rows wider than a workgroup holds, groups of one channel"""
+    from yolov5m_amd.group_norm import group_norm_act, group_norm_act_backward
+    shape, groups = case
+    x, dz = _rows(shape, "bf16", 60, offset=0.5), _rows(shape, "bf16", 61, scale=0.1)
+    ga, be = _params(shape[1], 62)
+    kept = None if keep == "x" else stored_values(x, keep)[0]
+    ref = Exact(x, groups, ga, be, 1e-3, "silu", kept, dz)
+    z, saved = group_norm_act(x, groups, ga, be, eps=1e-3, keep=keep)
+    ref.check(z, "z")
+    for got, what in zip(group_norm_act_backward(dz, saved), ("dx", "dgamma", "dbeta")):
+        ref.check(got, what)
+
+
+def test_more_samples_than_one_grid_dimension():
+    """33000 samples (the launches fold them over two dimensions of the grid), each long enough for the split form"""
+    if DEV != "cuda":
+        pytest.skip("34 million elements")
+    from yolov5m_amd.group_norm import group_norm_act, group_norm_act_backward
+    shape = (33000, 8, 128)
+    x, dz = _rows(shape, "bf16", 63, offset=0.5), _rows(shape, "bf16", 64, scale=0.1)
+    ga, be = _params(8, 65)
+    z, saved = group_norm_act(x, 2, ga, be, eps=1e-3, keep="x")
+    dx, dg, db = group_norm_act_backward(dz, saved)
+    ref = Exact(x, 2, ga, be, 1e-3, "silu", None, dz)
+    for got, what in ((z, "z"), (dx, "dx"), (dg, "dgamma"), (db, "dbeta")):
+        ref.check(got, what)
+
+
+@pytest.mark.parametrize("keep", ["x", "e4m3"])
+def test_outputs_larger_than_the_caches(keep):
+    """above 64 MB outputs are stored past the caches, by kernels of their own; the gradient in place of dz as well"""
+    if DEV != "cuda":
+        pytest.skip("34 million elements")
+    from yolov5m_amd import _lib
+    from yolov5m_amd.group_norm import group_norm_act, group_norm_act_backward
+    shape = (3, 96, 340, 351)
+    x, dz = _rows(shape, "bf16", 66, offset=0.5), _rows(shape, "bf16", 67, scale=0.1)
+    ga, be = _params(96, 68)
+    kept = None if keep == "x" else stored_values(x, keep)[0]
+    z, saved = group_norm_act(x, 32, ga, be, eps=1e-3, keep=keep)
+    dx, dg, db = group_norm_act_backward(dz, saved)
+    ref = Exact(x, 32, ga, be, 1e-3, "silu", kept, dz)
+    for got, what in ((z, "z"), (dx, "dx"), (dg, "dgamma"), (db, "dbeta")):
+        ref.check(got, what)
+    if keep == "x":
+        return
+    L, s, a = _lib.lib(), 340 * 351, saved.kept
+    ws = torch.empty(L.y5m_gn_act_bwd_workspace_bytes(3, s, 96, 32), dtype=torch.uint8, device=DEV)
+    _lib.check(L.y5m_gn_act_bwd(dz.data_ptr(), s * 96, 96, None, 0, 0, a.q.data_ptr(), a.q.shape[1], a.scale.data_ptr(), 1, ga.data_ptr(), be.data_ptr(),
+                                saved.mean.data_ptr(), saved.rstd.data_ptr(), 3, s, 96, 32, 1, dz.data_ptr(), s * 96, 96, None, None, ws.data_ptr(),
+                                ws.numel(), 1, _lib.stream_ptr()), "y5m_gn_act_bwd")
+    assert torch.equal(dz, dx)
+
+
+def test_offsets_beyond_32_bits():
+    """elements past 2^31: in the strides of the input and of dz, and in dense tensors (output, codes, gradient)"""
+    if DEV != "cuda":
+        pytest.skip("30 GB")
+    from yolov5m_amd.act8 import act8_load, act8_wgrad
+    from yolov5m_amd.group_norm import group_norm_act, group_norm_act_backward
+    ga, be = _params(64, 69)
+    wide = torch.empty((20000, 110000), dtype=torch.bfloat16, device=DEV)
+    x, dz = wide[:, 64:128].t()[None], wide[:, 109936:].t()[None]
+    x.copy_(_rows((1, 64, 20000), "bf16", 70, offset=0.5))
+    dz.copy_(_rows((1, 64, 20000), "bf16", 71, scale=0.1))
+    z, saved = group_norm_act(x, 4, ga, be, eps=1e-3, keep="x")
+    ref = Exact(x, 4, ga, be, 1e-3, "silu", None, dz)
+    ref.check(z, "z")
+    for got, what in zip(group_norm_act_backward(dz, saved), ("dx", "dgamma", "dbeta")):
+        ref.check(got, what)
+    del wide, x, dz, z, saved
+
+    shape = (140, 96, 400, 400)
+    ga, be = _params(96, 72)
+    big = lambda: torch.empty((140, 400, 400, 96), dtype=torch.bfloat16, device=DEV).normal_().movedim(-1, 1)
+    x, dz = big(), big()
+    z, saved = group_norm_act(x, 32, ga, be, eps=1e-3, keep="int8")
+    dx, dg, db = group_norm_act_backward(dz, saved)
+    y = act8_load(saved.kept)
+    for n in (0, 139):
+        kept = stored_values(x[n:n + 1], "int8")[0]
+        assert torch.equal(y[n:n + 1].cpu().movedim(1, -1).double(), kept)
+        ref = Exact(x[n:n + 1], 32, ga, be, 1e-3, "silu", kept, dz[n:n + 1])
+        ref.check(z[n:n + 1], "z")
+        ref.check(dx[n:n + 1], "dx")
+    # 22.4 million rows in 512 ranges of at most 43776: a wave's chain is a quarter of that in steps of 32, plus 32 products each
+    dw, dwb = act8_wgrad(dz, saved.kept, bias=True)
+    want, mag, sums, smag = (torch.zeros(s, dtype=torch.float64, device=DEV) for s in ((96, 96), (96, 96), (96,), (96,)))
+    for n in range(140):
+        d, v = dz[n].movedim(0, -1).reshape(-1, 96).double(), y[n].movedim(0, -1).reshape(-1, 96).double()
+        want += d.t() @ v
+        mag += d.abs().t() @ v.abs()
+        sums += d.sum(0)
+        smag += d.abs().sum(0)
+    assert ((dw.double() - want).abs() <= (342 + 32 + 8) * U * mag).all()
+    assert ((dwb.double() - sums).abs() <= (43776 // 16 + 16) * U * smag).all()
+
+
+def test_two_streams_at_once():
+    """the same operators on two streams at a time, several times over: each call has its own workspace, results equal the first ones"""
+    if DEV != "cuda":
+        pytest.skip("streams")
+    from yolov5m_amd.act8 import act8_wgrad
+    from yolov5m_amd.group_norm import group_norm_act, group_norm_act_backward
+    ga, be = _params(96, 73)
+
+    def step(x, dz):
+        z, saved = group_norm_act(x, 32, ga, be, keep="e4m3")
+        return (z, *group_norm_act_backward(dz, saved), *act8_wgrad(dz, saved.kept, bias=True))
+    data = [(_rows((n, 96, 80, 80), "bf16", 74 + n), _rows((n, 96, 80, 80), "bf16", 90 + n)) for n in (2, 8)]
+    want = [step(*d) for d in data]
+    side = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in side:
+        s.wait_stream(torch.cuda.current_stream())
+    got = []
+    for _ in range(4):
+        for s, d in zip(side, data):
+            with torch.cuda.stream(s):
+                got.append(step(*d))
+    torch.cuda.synchronize()
+    for i, out in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(want[i % 2], out)), i
+
+
+def test_empty_maps_of_any_layout():
+    from yolov5m_amd.act8 import act8_load, act8_store
+    from yolov5m_amd.group_norm import group_norm_act
+    for x in (torch.zeros((2, 8, 5, 0), device=DEV), torch.zeros((2, 8, 5, 0), device=DEV).contiguous(memory_format=torch.channels_last), torch.zeros((0, 8, 3), device=DEV)):
+        assert group_norm_act(x, 4)[0].shape == act8_load(act8_store(x)).shape == x.shape
+
+
+def test_a_kept_form_needs_group_norm():
+    from yolov5m_amd._lib import Y5MError
+    from yolov5m_amd.model import CBL
+    with pytest.raises(Y5MError, match="norm_groups"):
+        CBL(8, 8, 1, 1, 0, keep="int8")
