@@ -297,3 +297,18 @@ def test_wgrad_rows_far_apart():
     xv, dv = act8_load(kept).cpu().double()[0].t(), dy.cpu().double()[0].t()
     assert ((dw.cpu().double() - dv.t() @ xv).abs() <= 96 * U * (dv.abs().t() @ xv.abs())).all()
     assert ((db.cpu().double() - dv.sum(0)).abs() <= 160 * U * dv.abs().sum(0)).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "fp16"])
+@pytest.mark.parametrize("cout", [1, 2, 3, 4, 5, 7, 63, 65, 67])
+def test_wgrad_of_few_and_odd_channels(cout, dtype):
+    """pieces that end with the row, rows of less than one piece; rows at one distance and images apart"""
+    from yolov5m_amd.act8 import act8_load, act8_store, act8_wgrad
+    maps, wide = rows_tensor((3, 40, 9, 8), dtype, 18), rows_tensor((3, 80, 9, 8), dtype, 19, scale=0.1)
+    for x, dy in ((maps, wide[:, 3:3 + cout].contiguous(memory_format=torch.channels_last)), (maps, wide[:, 3:3 + cout]), (maps[:, :, 1:8], wide[:, 8:8 + cout, 1:8])):
+        kept = act8_store(x, "e4m3")
+        dw, db = act8_wgrad(dy, kept, bias=True)
+        xv = act8_load(kept).cpu().double().movedim(1, -1).reshape(-1, 40)
+        dv = dy.cpu().double().movedim(1, -1).reshape(-1, cout)
+        assert ((dw.cpu().double() - dv.t() @ xv).abs() <= 96 * U * (dv.abs().t() @ xv.abs())).all()
+        assert ((db.cpu().double() - dv.sum(0)).abs() <= 160 * U * dv.abs().sum(0)).all()

@@ -61,14 +61,24 @@ template <int ND> __device__ __forceinline__ void aw_buffer(__amdgpu_buffer_rsrc
     }
 }
 
-// FAST: rows at one distance, read in whole pieces through buffer resources that end with the range (the launcher keeps a range below
-// 2 GiB): rows beyond the range and channels beyond the last read as zero, the loop has no tail. Else element by element, any strides.
-template <int DT, int PA, int PC, bool FAST> struct AwLoader {
+// How rows are read.
+// AW_PIECES: rows at one distance, in whole pieces through buffer resources that end with the range (the launcher keeps a range below
+// 2 GiB): rows beyond the range and channels beyond the last read as zero, the loop has no tail.
+// AW_ROWS: rows at one distance that start at any element (codes and scales as above). A row's last piece is the PA values that END with
+// the row: its lane then holds `aw_shift` channels of its neighbour's as well, which are not stored. (Values shifted and masked
+// in the loop, rows addressed in 64 bits: 69 x 659 over 64152 rows in fp16 with the store of X 194 us, 84 so.)
+// AW_FEW: the same for fewer than PA channels, by elements (2 x 189 over 540676 rows in fp16 with the store: 224 us through AW_ANY, 115).
+// AW_ANY: any strides, any size.
+enum { AW_ANY = 0, AW_FEW = 1, AW_ROWS = 2, AW_PIECES = 3 };
+template <int MODE, int PA> __device__ __forceinline__ int aw_shift(int n, int N) {
+    return MODE != AW_PIECES && N >= PA && n < N && n + PA > N ? n + PA - N : 0;
+}
+template <int DT, int PA, int PC, int MODE> struct AwLoader {
     typedef typename RowElem<DT>::T T;
     static constexpr unsigned OOB = 0x80000000u;
     const AwParams& P;
     int64_t m0, m1;
-    int n, c, g;
+    int n, c, g, nl;
     bool nin, cin;
     __amdgpu_buffer_rsrc_t ry, rq, rs;
     unsigned ao, qo, so, as;                 // byte offsets of row 8 g (scales: of this lane's row) of the range, bytes from row to row of dY
@@ -78,36 +88,51 @@ template <int DT, int PA, int PC, bool FAST> struct AwLoader {
         : P(P_), m0(m0_), m1(m1_), n(n_), c(c_), g(g_) {
         nin = n < P.N;
         cin = c < P.C;
+        nl = nin && MODE != AW_FEW ? n - aw_shift<MODE, PA>(n, P.N) : 0;
         sr = 8 * g + (i16 & 7);
         sb = (c0 >> 5) + (i16 >> 3);
         sin = sb < P.CB;
         sin2 = PC == 8 && sb + 2 < P.CB;
-        if constexpr (FAST) {
+        if constexpr (MODE != AW_ANY) {
             as = (unsigned)(P.dr * (int64_t)sizeof(T));
             const unsigned rows = (unsigned)(m1 - m0);
-            ry = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(static_cast<const T*>(P.dy) + m0 * P.dr), 0, (rows - 1) * as + (unsigned)P.N * (unsigned)sizeof(T), 0x00020000);
+            if constexpr (MODE == AW_PIECES) ry = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(static_cast<const T*>(P.dy) + m0 * P.dr), 0, (rows - 1) * as + (unsigned)P.N * (unsigned)sizeof(T), 0x00020000);
             rq = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(P.q + m0 * P.ldq), 0, rows * (unsigned)P.ldq, 0x00020000);
             rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(P.scale + m0 * P.CB), 0, rows * (unsigned)P.CB, 0x00020000);
-            ao = nin ? (unsigned)(8 * g) * as + (unsigned)n * (unsigned)sizeof(T) : OOB;
+            ao = MODE != AW_PIECES ? (unsigned)nl * (unsigned)sizeof(T) : nin ? (unsigned)(8 * g) * as + (unsigned)n * (unsigned)sizeof(T) : OOB;
             qo = cin ? (unsigned)(8 * g) * (unsigned)P.ldq + (unsigned)c : OOB;
             so = (unsigned)sr * (unsigned)P.CB + (unsigned)sb;
         }
     }
     __device__ __forceinline__ void load(AwStage<DT, PA, PC>& st, unsigned step) const {       // step: rows from m0
         constexpr int AD = AwStage<DT, PA, PC>::AD;
-        if constexpr (FAST) {
+        if constexpr (MODE != AW_ANY) {
             const unsigned a = ao + step * as, q = qo + step * (unsigned)P.ldq, s = so + step * (unsigned)P.CB;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                aw_buffer<AD>(ry, a + (unsigned)j * as, st.a[j]);
+                if constexpr (MODE == AW_PIECES) {
+                    aw_buffer<AD>(ry, a + (unsigned)j * as, st.a[j]);
+                } else {
+                    const unsigned r = step + (unsigned)(8 * g + j);
+                    const bool in = r < (unsigned)(m1 - m0);
+                    const char* p = reinterpret_cast<const char*>(static_cast<const T*>(P.dy) + m0 * P.dr) + ((in ? r : 0u) * as + ao);
+                    if constexpr (MODE == AW_ROWS) {
+                        __builtin_memcpy(st.a[j], p, sizeof(st.a[j]));
+                    } else {
+                        T e[PA];
+#pragma unroll
+                        for (int k = 0; k < PA; ++k) e[k] = reinterpret_cast<const T*>(p)[k < P.N ? k : P.N - 1];
+                        __builtin_memcpy(st.a[j], e, sizeof(e));
+                    }
+#pragma unroll
+                    for (int k = 0; k < AD; ++k) st.a[j][k] = in ? st.a[j][k] : 0u;
+                }
                 aw_buffer<PC / 4>(rq, q + (unsigned)(j * P.ldq), st.q[j]);
             }
             st.s = __builtin_amdgcn_raw_buffer_load_b8(rs, sin ? s : OOB, 0, 0);
             if constexpr (PC == 8) st.s2 = __builtin_amdgcn_raw_buffer_load_b8(rs, sin2 ? s + 2 : OOB, 0, 0);
         } else {
-            // rows that start anywhere (the compiler's unaligned vector loads). A row's last piece is the PA values that END with the
-            // row, shifted down, so that no lane branches around a load; N < PA by elements. P.S = 0: the rows at one distance
-            const int sh = nin && n + PA > P.N ? n + PA - P.N : 0, nl = nin ? n - sh : 0;
+            // N < PA by elements. P.S = 0: the rows at one distance
             const bool small = P.N < PA;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -121,18 +146,13 @@ template <int DT, int PA, int PC, bool FAST> struct AwLoader {
                     for (int k = 0; k < PA; ++k) e[k] = p[n + k < P.N ? n + k : P.N - 1];
                 } else {
                     __builtin_memcpy(e, p + nl, sizeof(e));
-#pragma unroll
-                    for (int s2 = PA / 2; s2 > 0; s2 >>= 1)
-#pragma unroll
-                        for (int k = 0; k + s2 < PA; ++k) e[k] = (sh & s2) ? e[k + s2] : e[k];
                 }
                 if constexpr (DT == Y5M_F32) {
 #pragma unroll
-                    for (int k = 0; k < PA; ++k) st.a[j][k] = in && n + k < P.N ? __float_as_uint(e[k]) : 0u;
+                    for (int k = 0; k < PA; ++k) st.a[j][k] = in ? __float_as_uint(e[k]) : 0u;
                 } else {
 #pragma unroll
-                    for (int k = 0; k < PA / 2; ++k)
-                        st.a[j][k] = (in && n + 2 * k < P.N ? (unsigned)e[2 * k] : 0u) | (in && n + 2 * k + 1 < P.N ? (unsigned)e[2 * k + 1] << 16 : 0u);
+                    for (int k = 0; k < PA / 2; ++k) st.a[j][k] = in ? (unsigned)e[2 * k] | (unsigned)e[2 * k + 1] << 16 : 0u;
                 }
                 const uint8_t* q = P.q + r * P.ldq + (cin ? c : 0);
 #pragma unroll
@@ -167,7 +187,7 @@ template <int FMT> __device__ __forceinline__ unsigned aw_decode2(unsigned w, fl
     }
 }
 
-template <int DT, int FMT, int PA, int PC, int WN, int WC, int WK, bool FAST, bool DB>
+template <int DT, int FMT, int PA, int PC, int WN, int WC, int WK, int MODE, bool DB>
 __global__ __launch_bounds__(AW_THREADS, PA * PC <= 32 ? 2 : 1) void act8_wgrad_kernel(const AwParams P) {
     static_assert(WN * WC * WK == AW_THREADS / 64, "four waves");
     constexpr int NP = AwPieces<DT>::n;
@@ -193,7 +213,7 @@ __global__ __launch_bounds__(AW_THREADS, PA * PC <= 32 ? 2 : 1) void act8_wgrad_
 #pragma unroll
     for (int k = 0; k < PA; ++k) bias[k] = 0.f;
 
-    const AwLoader<DT, PA, PC, FAST> L(P, m0, m1, n0 + PA * i16, c0 + PC * i16, g, c0, i16);
+    const AwLoader<DT, PA, PC, MODE> L(P, m0, m1, n0 + PA * i16, c0 + PC * i16, g, c0, i16);
     auto compute = [&](AwStage<DT, PA, PC>& st) __attribute__((always_inline)) {
         // (rows and channels beyond the last: codes 0, scale byte 0 = 0.0)
         aw_bf16x8 xf[PC];
@@ -318,8 +338,10 @@ __global__ __launch_bounds__(AW_THREADS, PA * PC <= 32 ? 2 : 1) void act8_wgrad_
     if constexpr (DB) {
         __syncthreads();
         if (ct == 0 && wc == 0 && g == 0) {
+            const int sh = aw_shift<MODE, PA>(n0 + PA * i16, P.N);
 #pragma unroll
-            for (int k = 0; k < PA; ++k) redb[(wk * WN + wn) * 16 * PA + PA * i16 + k] = bias[k];
+            for (int k = 0; k < PA; ++k)
+                if (k >= sh) redb[(wk * WN + wn) * 16 * PA + PA * i16 + k - sh] = bias[k];
         }
         __syncthreads();
         const int nn = nt * WN * 16 * PA + tid;
@@ -339,8 +361,8 @@ __global__ __launch_bounds__(AW_THREADS, PA * PC <= 32 ? 2 : 1) void act8_wgrad_
         for (int ja = 0; ja < PA; ++ja)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int n = n0 + PA * (4 * g + r) + ja;
-                if (n >= P.N) continue;
+                const int np = n0 + PA * (4 * g + r), sh = aw_shift<MODE, PA>(np, P.N), n = np + ja - sh;
+                if (n >= P.N || ja < sh) continue;
                 float* d = part + (size_t)n * P.C + c;
 #pragma unroll
                 for (int h = 0; h < PC / 4; ++h) {
@@ -428,29 +450,29 @@ extern "C" size_t y5m_act8_wgrad_workspace_bytes(int64_t M, int Cout, int C) {
     return (size_t)(a > P.ranges ? a : P.ranges) * ((size_t)Cout * C + Cout) * sizeof(float);
 }
 
-template <int DT, int FMT, int PA, int PC, int WN, int WC, bool FAST, bool DB>
+template <int DT, int FMT, int PA, int PC, int WN, int WC, int MODE, bool DB>
 static int aw_launch_db(const AwParams& P, hipStream_t st) {
     constexpr int WK = 4 / (WN * WC), lds = ((WK - 1) * WN * WC * (PA / 2 * PC * 4) * 64 + WK * WN * 16 * PA) * (int)sizeof(float);
     static_assert(lds <= 160 * 1024, "LDS");
     static std::atomic<uint64_t> asked{0};
-    if (!lds_ask(reinterpret_cast<const void*>(act8_wgrad_kernel<DT, FMT, PA, PC, WN, WC, WK, FAST, DB>), lds, lds, asked)) return Y5M_ELAUNCH;
-    hipLaunchKernelGGL((act8_wgrad_kernel<DT, FMT, PA, PC, WN, WC, WK, FAST, DB>), dim3((unsigned)((int64_t)P.tiles_n * P.tiles_c * P.ranges)), dim3(AW_THREADS), lds, st, P);
+    if (!lds_ask(reinterpret_cast<const void*>(act8_wgrad_kernel<DT, FMT, PA, PC, WN, WC, WK, MODE, DB>), lds, lds, asked)) return Y5M_ELAUNCH;
+    hipLaunchKernelGGL((act8_wgrad_kernel<DT, FMT, PA, PC, WN, WC, WK, MODE, DB>), dim3((unsigned)((int64_t)P.tiles_n * P.tiles_c * P.ranges)), dim3(AW_THREADS), lds, st, P);
     Y5M_CHECK_LAUNCH("act8_wgrad_kernel");
     return Y5M_OK;
 }
-template <int DT, int FMT, int PA, int PC, int WN, int WC, bool FAST> static int aw_launch(const AwParams& P, hipStream_t st) {
-    return P.dbpart ? aw_launch_db<DT, FMT, PA, PC, WN, WC, FAST, true>(P, st) : aw_launch_db<DT, FMT, PA, PC, WN, WC, FAST, false>(P, st);
+template <int DT, int FMT, int PA, int PC, int WN, int WC, int MODE> static int aw_launch(const AwParams& P, hipStream_t st) {
+    return P.dbpart ? aw_launch_db<DT, FMT, PA, PC, WN, WC, MODE, true>(P, st) : aw_launch_db<DT, FMT, PA, PC, WN, WC, MODE, false>(P, st);
 }
-template <int FMT> static int aw_dispatch(const AwParams& P, const AwShape& s, int dtype, bool fast, hipStream_t st) {
-    constexpr int B = Y5M_BF16, H = Y5M_F16, F = Y5M_F32;
-    if (s.pa == 4 && s.pc == 4) {
-        if (dtype == F) return fast ? aw_launch<F, FMT, 4, 4, 1, 1, true>(P, st) : aw_launch<F, FMT, 4, 4, 1, 1, false>(P, st);
-        if (dtype == H) return fast ? aw_launch<H, FMT, 4, 4, 1, 1, true>(P, st) : aw_launch<H, FMT, 4, 4, 1, 1, false>(P, st);
-        return fast ? aw_launch<B, FMT, 4, 4, 1, 1, true>(P, st) : aw_launch<B, FMT, 4, 4, 1, 1, false>(P, st);
-    }
-    if (s.pa == 4) return aw_launch<B, FMT, 4, 8, 1, 1, true>(P, st);
-    if (s.wn == 2) return aw_launch<B, FMT, 8, 8, 2, 1, true>(P, st);
-    return s.wc == 2 ? aw_launch<B, FMT, 8, 8, 1, 2, true>(P, st) : aw_launch<B, FMT, 8, 8, 1, 1, true>(P, st);
+template <int DT, int FMT> static int aw_small(const AwParams& P, int mode, hipStream_t st) {
+    return mode == AW_PIECES ? aw_launch<DT, FMT, 4, 4, 1, 1, AW_PIECES>(P, st) : mode == AW_ROWS ? aw_launch<DT, FMT, 4, 4, 1, 1, AW_ROWS>(P, st)
+           : mode == AW_FEW ? aw_launch<DT, FMT, 4, 4, 1, 1, AW_FEW>(P, st) : aw_launch<DT, FMT, 4, 4, 1, 1, AW_ANY>(P, st);
+}
+template <int FMT> static int aw_dispatch(const AwParams& P, const AwShape& s, int dtype, int mode, hipStream_t st) {
+    constexpr int B = Y5M_BF16;
+    if (s.pa == 4 && s.pc == 4) return dtype == Y5M_F32 ? aw_small<Y5M_F32, FMT>(P, mode, st) : dtype == Y5M_F16 ? aw_small<Y5M_F16, FMT>(P, mode, st) : aw_small<B, FMT>(P, mode, st);
+    if (s.pa == 4) return aw_launch<B, FMT, 4, 8, 1, 1, AW_PIECES>(P, st);
+    if (s.wn == 2) return aw_launch<B, FMT, 8, 8, 2, 1, AW_PIECES>(P, st);
+    return s.wc == 2 ? aw_launch<B, FMT, 8, 8, 1, 2, AW_PIECES>(P, st) : aw_launch<B, FMT, 8, 8, 1, 1, AW_PIECES>(P, st);
 }
 
 extern "C" int y5m_act8_wgrad(const void* dy, int64_t dy_batch_stride, int64_t dy_row_stride, int64_t N, int64_t S, int Cout, const void* q, int ldq,
@@ -470,12 +492,13 @@ extern "C" int y5m_act8_wgrad(const void* dy, int64_t dy_batch_stride, int64_t d
     // rows of all samples at one distance in whole vector pieces, and a range of them within a buffer resource's 32-bit offsets
     const int64_t pitch = S == 1 && N > 1 ? dy_batch_stride : dy_row_stride;      // (one row per sample: the samples are the rows)
     const bool flat = N == 1 || S == 1 || dy_batch_stride == S * dy_row_stride;
-    bool fast = flat && rows_aligned16(dy, dy_batch_stride, dy_row_stride, N, S, Cout, dtype) && pitch >= Cout && pitch < (1 << 24);
+    const bool near = flat && pitch >= 0 && pitch < (1 << 24);
+    int mode = near && pitch >= Cout && rows_aligned16(dy, dy_batch_stride, dy_row_stride, N, S, Cout, dtype) ? AW_PIECES : near ? (Cout >= 4 ? AW_ROWS : AW_FEW) : AW_ANY;
     AwParams P = {};
-    AwShape s = aw_shape(Cout, C, fast && dtype == Y5M_BF16);
+    AwShape s = aw_shape(Cout, C, mode == AW_PIECES && dtype == Y5M_BF16);
     aw_geometry(P, s, N * S, Cout, C);
-    if (fast && (P.per + 4 * AW_K * s.wk) * (pitch > ldq ? pitch : ldq) * (dtype == Y5M_F32 ? 4 : 2) >= (1ll << 31)) {
-        fast = false;
+    if (mode != AW_ANY && (P.per + 4 * AW_K * s.wk) * (pitch > ldq ? pitch : ldq) * (dtype == Y5M_F32 ? 4 : 2) >= (1ll << 31)) {
+        mode = AW_ANY;
         s = aw_shape(Cout, C, false);
         aw_geometry(P, s, N * S, Cout, C);
     }
@@ -485,7 +508,7 @@ extern "C" int y5m_act8_wgrad(const void* dy, int64_t dy_batch_stride, int64_t d
     P.dbpart = db ? P.part + (size_t)P.ranges * Cout * C : nullptr;
     P.dw = dw; P.db = db;
     Y5M_REQUIRE((int64_t)P.tiles_n * P.tiles_c * P.ranges < (1ll << 24) && (int64_t)Cout * C * P.slots < (1ll << 31), "too many workgroups");
-    const int rc = fmt == Y5M_KEEP_E4M3 ? aw_dispatch<Y5M_KEEP_E4M3>(P, s, dtype, fast, y5m_stream(stream)) : aw_dispatch<Y5M_KEEP_INT8>(P, s, dtype, fast, y5m_stream(stream));
+    const int rc = fmt == Y5M_KEEP_E4M3 ? aw_dispatch<Y5M_KEEP_E4M3>(P, s, dtype, mode, y5m_stream(stream)) : aw_dispatch<Y5M_KEEP_INT8>(P, s, dtype, mode, y5m_stream(stream));
     if (rc != Y5M_OK) return rc;
     const int64_t items = (int64_t)Cout * C + (db ? Cout : 0), per = AW_THREADS / P.slots;
     hipLaunchKernelGGL(act8_wgrad_join_kernel, dim3((unsigned)((items + per - 1) / per)), dim3(AW_THREADS), 0, y5m_stream(stream), P);
