@@ -451,7 +451,8 @@ int y5m_adam_step(float* p, const float* g, float* m, float* v, int64_t n, const
 int y5m_act8_store(const void* x, int64_t x_batch_stride, int64_t x_row_stride, int64_t N, int64_t S, int C, void* q, int ldq,
                    void* scale, int fmt, int dtype, void* stream);
 int y5m_act8_load(const void* q, int ldq, const void* scale, int64_t M, int C, void* x, int64_t x_row_stride, int fmt, int dtype,
-                  void* stream);/* weight gradient of a pointwise convolution from its input in 8 bits: dw[n][c] = sum over the N * S rows of dy[row][n] * value[row][c]
+                  void* stream);
+/* weight gradient of a pointwise convolution from its input in 8 bits: dw[n][c] = sum over the N * S rows of dy[row][n] * value[row][c]
  * (f32, [Cout][C], OVERWRITTEN); db[n] = sum of dy[row][n] (NULL: not wanted). dtype: dy's. No atomics, one result per input. */
 size_t y5m_act8_wgrad_workspace_bytes(int64_t M, int Cout, int C);
 int y5m_act8_wgrad(const void* dy, int64_t dy_batch_stride, int64_t dy_row_stride, int64_t N, int64_t S, int Cout, const void* q, int ldq,

@@ -222,41 +222,45 @@ __device__ __forceinline__ double gn_wave_sum(double v) {
     return v;
 }
 // a workgroup's sum of NV doubles per thread, in a fixed order; every thread gets it
-template <int NV> __device__ __forceinline__ void gn_block_sum(double* v, double* red) {
+template <int NV, int T> __device__ __forceinline__ void gn_block_sum(double* v, double* red) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) v[i] = gn_wave_sum(v[i]);
     if ((threadIdx.x & 63) == 0) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) red[i * 4 + (threadIdx.x >> 6)] = v[i];
+        for (int i = 0; i < NV; ++i) red[i * (T / 64) + (threadIdx.x >> 6)] = v[i];
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < NV; ++i) v[i] = (red[i * 4] + red[i * 4 + 1]) + (red[i * 4 + 2] + red[i * 4 + 3]);
+    for (int i = 0; i < NV; ++i) {
+        v[i] = 0.0;
+        for (int k = 0; k < T / 64; k += 4) v[i] += (red[i * (T / 64) + k] + red[i * (T / 64) + k + 1]) + (red[i * (T / 64) + k + 2] + red[i * (T / 64) + k + 3]);
+    }
     __syncthreads();
 }
-// One workgroup per (sample, group): its chunks x D channels are walked over in pieces of w = min(D, 256) channels, 256 / w chunks side
-// by side. (Latency is all there is: four loads in flight per thread, 4 us where one wave per group took 7.)
+// One workgroup of T threads per (sample, group): its chunks x D channels are walked over in pieces of w = min(D, T) channels, T / w
+// chunks side by side. (Latency is all there is: four loads in flight per thread, 4 us where one wave per group took 7.) T = 1024 where a
+// group has many channels and chunks.
 struct GnWalk { int w, slots, slot, d; };
-__device__ __forceinline__ GnWalk gn_walk(int D) {
+template <int T> __device__ __forceinline__ GnWalk gn_walk(int D) {
     GnWalk k;
-    k.w = D < GN_THREADS ? D : GN_THREADS;
-    k.slots = GN_THREADS / k.w;
+    k.w = D < T ? D : T;
+    k.slots = T / k.w;
     k.slot = (int)threadIdx.x / k.w;
     k.d = (int)threadIdx.x - k.slot * k.w;
     return k;
 }
 
-__global__ __launch_bounds__(GN_THREADS) void gn_stats_join_kernel(const GnParams P) {
-    __shared__ double red[12];
+template <int T> __global__ __launch_bounds__(T) void gn_stats_join_kernel(const GnParams P) {
+    __shared__ double red[3 * T / 64];
     const int64_t b = (int64_t)blockIdx.z * gridDim.y + blockIdx.y;
     const int g = (int)blockIdx.x;
     if (b >= P.N) return;
     const float* part = P.part + (size_t)b * P.chunks * 2 * P.C + 2 * g * P.D;
-    const GnWalk k = gn_walk(P.D);
+    const GnWalk k = gn_walk<T>(P.D);
     const double ref = (double)part[0];
     double v[3] = {0.0, 0.0, 0.0};                                 // sum R (m - ref), sum R (m - ref)^2, sum M2
     if (k.slot < k.slots)
-        for (int d = k.d; d < P.D; d += GN_THREADS) {
+        for (int d = k.d; d < P.D; d += T) {
             auto add = [&](const float2& m, int ch) __attribute__((always_inline)) {
                 const double R = (double)(ch + 1 < P.chunks ? P.rpc : P.S - ch * P.rpc), e = (double)m.x - ref;
                 v[0] += R * e;
@@ -273,7 +277,7 @@ __global__ __launch_bounds__(GN_THREADS) void gn_stats_join_kernel(const GnParam
             }
             for (; ch < P.chunks; ch += k.slots) add(*reinterpret_cast<const float2*>(part + (size_t)ch * 2 * P.C + 2 * d), ch);
         }
-    gn_block_sum<3>(v, red);
+    gn_block_sum<3, T>(v, red);
     if (threadIdx.x == 0) {
         const double off = v[0] * P.inv_k;
         double var = (v[2] + v[1]) * P.inv_k - off * off;
@@ -558,15 +562,15 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_reduce_kernel(const GnParam
 }
 
 // channel sums of a sample and A, B of its groups, one workgroup per (sample, group)
-__global__ __launch_bounds__(GN_THREADS) void gn_bwd_join_kernel(const GnParams P) {
-    __shared__ double red[2 * GN_THREADS];
+template <int T> __global__ __launch_bounds__(T) void gn_bwd_join_kernel(const GnParams P) {
+    __shared__ double red[2 * T];
     const int64_t n = (int64_t)blockIdx.z * gridDim.y + blockIdx.y;
     const int g = (int)blockIdx.x;
     if (n >= P.N) return;
     const float* part = P.part + (size_t)n * P.chunks * 2 * P.C + 2 * g * P.D;
-    const GnWalk k = gn_walk(P.D);
+    const GnWalk k = gn_walk<T>(P.D);
     double v[2] = {0.0, 0.0};
-    for (int d0 = 0; d0 < P.D; d0 += GN_THREADS) {                 // (uniform: every thread meets at the barriers)
+    for (int d0 = 0; d0 < P.D; d0 += T) {                 // (uniform: every thread meets at the barriers)
         const int d = d0 + k.d;
         const bool in = k.slot < k.slots && d < P.D;
         double s0 = 0.0, s1 = 0.0;
@@ -586,12 +590,12 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_join_kernel(const GnParams 
             }
         }
         red[threadIdx.x] = s0;
-        red[GN_THREADS + threadIdx.x] = s1;
+        red[T + threadIdx.x] = s1;
         __syncthreads();
         if (in && k.slot == 0) {
             for (int sl = 1; sl < k.slots; ++sl) {
                 s0 += red[sl * k.w + k.d];
-                s1 += red[GN_THREADS + sl * k.w + k.d];
+                s1 += red[T + sl * k.w + k.d];
             }
             const int c = g * P.D + d;
             *reinterpret_cast<float2*>(P.nc + ((size_t)n * P.C + c) * 2) = make_float2((float)s0, (float)s1);
@@ -601,7 +605,7 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_join_kernel(const GnParams 
         }
         __syncthreads();
     }
-    gn_block_sum<2>(v, red);
+    gn_block_sum<2, T>(v, red);
     if (threadIdx.x == 0) {
         *reinterpret_cast<float2*>(P.ab + (n * P.G + g) * 2) = make_float2((float)(v[0] * P.inv_k), (float)(v[1] * P.inv_k));
     }
@@ -997,9 +1001,13 @@ static int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // split: column tiles of at most GN_THREADS pieces; row chunks of 16 rows a thread in the reduce pass (whose sums are then joined), of 8
 // in the apply pass (short workgroups: 10000 of them stream at 6 TB/s, 2048 long ones at 5). 8 / 16, 12 / 12, 24 / 24 and 16 / 48 were 2 to
 // 9 % slower over the 40 x 40, 80 x 80 and 160 x 160 training steps at batch 64. At most 65536 chunks in all, so that the sums stay small
-// against the rows.
+// against the rows. Below two workgroups per CU the chunks are shorter, down to 4 rows a thread (what a thread does in turn is all the
+// time there is: the backward of one 80 x 80 x 96 map 20.7 -> 16.1 us, of four 22.5 -> 19.7; 2 rows gain where one map is small, 15.1,
+// and lose at two to eight), unless the joins would grow beyond 4096 pairs a group (2 groups of 693 channels, 155 rows: 24.5 -> 29).
+// A group of GN_WIDE pairs or more is joined by 1024 threads (one group of 768 channels, 2500 rows: forward 38 -> 24.5).
 #define GN_ROWS 16
 #define GN_APPLY_ROWS 8
+#define GN_WIDE 4096
 static void gn_geometry(GnParams& P, bool quads, int rows, int arows) {
     P.CB = (P.C + 31) / 32;
     P.CV = quads ? P.CB * 4 : (P.C + 7) / 8;
@@ -1008,6 +1016,7 @@ static void gn_geometry(GnParams& P, bool quads, int rows, int arows) {
     if (quads) P.ct = (P.ct + 3) / 4 * 4;
     P.RP = GN_THREADS / P.ct;
     auto cut = [&](int rows, int& chunks, int& rpc) {
+        while (rows > 4 && P.N * P.tiles * ceil_div(P.S, (int64_t)P.RP * rows) < 512 && ceil_div(P.S, (int64_t)P.RP * rows / 2) * P.D <= 4096) rows /= 2;
         int64_t c = ceil_div(P.S, (int64_t)P.RP * rows), cap = ceil_div(65536, P.N);
         if (c > cap) c = cap;
         rpc = (int)(ceil_div(ceil_div(P.S, c), P.RP) * P.RP);
@@ -1022,7 +1031,8 @@ static void gn_geometry(GnParams& P, bool quads, int rows, int arows) {
 // ascending; `most`: elements in all, above which the split form is faster -- except for samples of few rows, whose chunks would be
 // scraps. Held against split, 20 x 20 x 768 bf16 in 32 groups: forward of 1 / 16 / 32 / 64 images 9 / 14 / 17 / 30 us against 14 / 18 / 23 / 32,
 // of 256 165 against 105; backward of 1 / 8 / 16 / 32 images 13 / 14 / 23 / 39 against 21 / 24 / 29 / 36. 16384 x 768 tokens (one row
-// each): forward 92 against 940.
+// each): forward 92 against 940. 16 rows a thread pay from 128 workgroups on: 64 / 128 / 256 of them (40 x 40, 96 and 192 channels) 13.4 /
+// 14.6 / 17.4 against 12.1 / 14.8 / 24.1; three of one channel per group, 7623 rows: 28.4 against 12.6.
 struct GnHeld { int threads, nr; };
 static GnHeld gn_held(GnParams& P, bool blocks, bool aligned, const int* nrs, int64_t most) {
     // whole groups, whole blocks or pieces; rows that start anywhere may be cut anywhere (at 8 channels or more: load_raw8)
@@ -1054,6 +1064,7 @@ static GnHeld gn_held(GnParams& P, bool blocks, bool aligned, const int* nrs, in
         ++k;
     }
     if (h.nr == 0 || (P.N * P.S * P.C > most && P.S >= 128)) return {0, 0};
+    if (h.nr > 4 && P.N * ceil_div(units, k) < 128) return {0, 0};
     if (P.N * ceil_div(units, k) * h.threads >= (1ll << 32)) return {0, 0};          // (the launch's threads are counted in 32 bits)
     P.sc = (int64_t)unit * k < P.C ? unit * k : P.C;
     P.slices = (int)ceil_div(P.C, P.sc);
@@ -1103,12 +1114,17 @@ static dim3 gn_grid(int64_t x, int64_t N) {
     return dim3((unsigned)x, (unsigned)y, (unsigned)ceil_div(N, y));
 }
 // (at most 65536 chunks of 32 tiles, or 65535 groups: every dimension is below 2^24 workgroups = 2^32 threads)
+#define GN_JOINS(K)                                                                                                          \
+    do {                                                                                                                     \
+        if ((int64_t)P.chunks * P.D >= GN_WIDE) hipLaunchKernelGGL(K<1024>, gn_grid(P.G, P.N), dim3(1024), 0, st, P);        \
+        else hipLaunchKernelGGL(K<GN_THREADS>, gn_grid(P.G, P.N), dim3(GN_THREADS), 0, st, P);                               \
+    } while (0)
 #define GN_LAUNCH2(K, x) hipLaunchKernelGGL(K, gn_grid((int64_t)(x), P.N), dim3(GN_THREADS), 0, st, P)
 
 template <int DT, int AL, int FMT> static int gn_fwd_split(GnParams& P, hipStream_t st) {
     gn_geometry(P, FMT != Y5M_KEEP_NONE, GN_ROWS, GN_APPLY_ROWS);
     GN_LAUNCH2((gn_stats_kernel<DT, AL>), P.chunks * P.tiles);
-    GN_LAUNCH2(gn_stats_join_kernel, P.G);
+    GN_JOINS(gn_stats_join_kernel);
     if constexpr (AL > 0) {
         if (rows_past_caches(P.N * P.S, P.C, DT)) GN_LAUNCH2((gn_apply_kernel<DT, 2, FMT>), P.achunks * P.tiles);
         else GN_LAUNCH2((gn_apply_kernel<DT, 1, FMT>), P.achunks * P.tiles);
@@ -1177,7 +1193,7 @@ template <int DT, int AL, int FMT> static int gn_bwd(GnParams& P, hipStream_t st
     } else {
         gn_geometry(P, false, GN_ROWS, GN_APPLY_ROWS);
                 GN_LAUNCH2((gn_bwd_reduce_kernel<DT, AL, FMT>), P.chunks * P.tiles);
-        GN_LAUNCH2(gn_bwd_join_kernel, P.G);
+        GN_JOINS(gn_bwd_join_kernel);
         if constexpr (AL > 0) {
             if (rows_past_caches(P.N * P.S, P.C, DT)) GN_LAUNCH2((gn_bwd_apply_kernel<DT, 2, FMT>), P.achunks * P.tiles);
             else GN_LAUNCH2((gn_bwd_apply_kernel<DT, 1, FMT>), P.achunks * P.tiles);
