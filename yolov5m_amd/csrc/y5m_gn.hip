@@ -9,7 +9,8 @@
 //   held (gn_held_*): a workgroup loads all rows of a slice of whole groups of one sample into registers, reduces, applies, stores: every
 //     byte is touched once, one launch (the backward's sums over the samples take a second, small one). For small maps, where launches
 //     are what costs;
-//   split: a reduce pass over row chunks, a small launch that joins the chunks in f64, an apply pass that reads the rows again.
+//   split: a reduce pass over row chunks, a small launch that joins the chunks in f64 (few of them: the apply pass does it), an apply
+//     pass that reads the rows again.
 // Neither uses atomics: the result does not depend on the order in which workgroups run. What else was built and measured, at
 // 64 x 160 x 160 x 96 in bf16 with the int8 form (forward + backward): one launch whose workgroups wait for each other's sums (their
 // round trips past the L2s and the registers of the join cost more than the second read: 604 us at best), batches of samples whose
@@ -250,6 +251,20 @@ template <int T> __device__ __forceinline__ GnWalk gn_walk(int D) {
     return k;
 }
 
+// a group's mean and rstd from its chunks' sums about ref: sum R (m - ref), sum R (m - ref)^2, sum M2
+__device__ __forceinline__ float2 gn_group_stat(const GnParams& P, const double* v, double ref) {
+    const double off = v[0] * P.inv_k;
+    double var = (v[2] + v[1]) * P.inv_k - off * off;
+    if (!(var > 0.0) && var == var) var = 0.0;                     // (a NaN stays)
+    return make_float2((float)(ref + off), 1.0f / sqrtf((float)(var + (double)P.eps)));
+}
+__device__ __forceinline__ void gn_add_chunk(const GnParams& P, const float2& m, int ch, double ref, double* v) {
+    const double R = (double)(ch + 1 < P.chunks ? P.rpc : P.S - ch * P.rpc), e = (double)m.x - ref;
+    v[0] += R * e;
+    v[1] += R * e * e;
+    v[2] += (double)m.y;
+}
+
 template <int T> __global__ __launch_bounds__(T) void gn_stats_join_kernel(const GnParams P) {
     __shared__ double red[3 * T / 64];
     const int64_t b = (int64_t)blockIdx.z * gridDim.y + blockIdx.y;
@@ -258,15 +273,10 @@ template <int T> __global__ __launch_bounds__(T) void gn_stats_join_kernel(const
     const float* part = P.part + (size_t)b * P.chunks * 2 * P.C + 2 * g * P.D;
     const GnWalk k = gn_walk<T>(P.D);
     const double ref = (double)part[0];
-    double v[3] = {0.0, 0.0, 0.0};                                 // sum R (m - ref), sum R (m - ref)^2, sum M2
+    double v[3] = {0.0, 0.0, 0.0};
     if (k.slot < k.slots)
         for (int d = k.d; d < P.D; d += T) {
-            auto add = [&](const float2& m, int ch) __attribute__((always_inline)) {
-                const double R = (double)(ch + 1 < P.chunks ? P.rpc : P.S - ch * P.rpc), e = (double)m.x - ref;
-                v[0] += R * e;
-                v[1] += R * e * e;
-                v[2] += (double)m.y;
-            };
+            auto add = [&](const float2& m, int ch) __attribute__((always_inline)) { gn_add_chunk(P, m, ch, ref, v); };
             int ch = k.slot;
             for (; ch + 3 * k.slots < P.chunks; ch += 4 * k.slots) {
                 float2 m[4];
@@ -279,12 +289,42 @@ template <int T> __global__ __launch_bounds__(T) void gn_stats_join_kernel(const
         }
     gn_block_sum<3, T>(v, red);
     if (threadIdx.x == 0) {
-        const double off = v[0] * P.inv_k;
-        double var = (v[2] + v[1]) * P.inv_k - off * off;
-        if (!(var > 0.0) && var == var) var = 0.0;                 // (a NaN stays)
+        const float2 st = gn_group_stat(P, v, ref);
         const int64_t ng = b * P.G + g;
-        P.mean[ng] = (float)(ref + off);
-        P.rstd[ng] = 1.0f / sqrtf((float)(var + (double)P.eps));
+        P.mean[ng] = st.x;
+        P.rstd[ng] = st.y;
+    }
+}
+
+// The same in the prologue of the apply passes, where the sums are few (gn_inline): every workgroup joins the groups that its tile
+// touches, k lanes a group, and saves the launch. val(g, chunk, channel of the group, pair of sums, v) adds, f(g, v) takes the result.
+template <int NV, typename V, typename F> __device__ __forceinline__ void gn_tile_groups(const GnParams& P, const GnPlace& w, int g0, int g1, V val, F f) {
+    int k = 64;
+    while ((g1 - g0 + 1) * k > GN_THREADS && k > 1) k >>= 1;
+    const int sub = threadIdx.x & (k - 1), pairs = P.chunks * P.D;
+    const float2* part = reinterpret_cast<const float2*>(P.part) + (size_t)w.n * P.chunks * P.C;
+    for (int g = g0 + (int)threadIdx.x / k; g <= g1; g += GN_THREADS / k) {
+        double v[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i] = 0.0;
+        for (int i = sub; i < pairs; i += 4 * k) {
+            float2 m[4];
+            int ch[4], d[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int j = i + u * k < pairs ? i + u * k : pairs - 1;
+                ch[u] = gn_div(j, P.dm);
+                d[u] = j - ch[u] * P.D;
+                m[u] = part[(size_t)ch[u] * P.C + g * P.D + d[u]];
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (i + u * k < pairs) val(g, ch[u], d[u], m[u], v);
+        }
+        for (int o = k >> 1; o > 0; o >>= 1)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) v[i] += gn_shfl_xor(v[i], o);
+        if (sub == 0) f(g, v);
     }
 }
 
@@ -306,11 +346,14 @@ __device__ __forceinline__ void gn_stat8(const GnParams& P, const GnPlace& w, co
         k.rstd[i] = P.rstd[w.n * P.G + gr.g[i]];
     }
 }
-__device__ __forceinline__ void gn_coef(const GnParams& P, const GnPlace& w, const GnGroups& gr, GnCoef& k) {
-    gn_stat8(P, w, gr, k);
+__device__ __forceinline__ void gn_param(const GnParams& P, const GnPlace& w, GnCoef& k) {
     const int c = w.in ? w.c : 0, nv = w.in ? w.nv : P.C;
     gn_param8(P.gamma, c, nv, 1.0f, k.gamma);
     gn_param8(P.beta, c, nv, 0.0f, k.beta);
+}
+__device__ __forceinline__ void gn_coef(const GnParams& P, const GnPlace& w, const GnGroups& gr, GnCoef& k) {
+    gn_stat8(P, w, gr, k);
+    gn_param(P, w, k);
 }
 
 // t = gamma xhat + beta. f32: (x - mean) first, exact where x is near the mean. 16 bits: one fma, x a + b -- its rounding of |mean| a
@@ -331,7 +374,7 @@ template <int DT> struct GnAffine {
     }
 };
 
-template <int DT, int AL, int FMT>
+template <int DT, int AL, int FMT, bool INL>
 __global__ __launch_bounds__(GN_THREADS) void gn_apply_kernel(const GnParams P) {
     typedef typename RowElem<DT>::T T;
     const GnPlace w = gn_place<true>(P, P.arpc);
@@ -340,7 +383,31 @@ __global__ __launch_bounds__(GN_THREADS) void gn_apply_kernel(const GnParams P) 
     GnAffine<DT> af;
     {
         GnCoef k;
-        gn_coef(P, w, gr, k);
+        if constexpr (INL) {
+            __shared__ float2 stat[GN_THREADS];
+            const int c0 = (w.piece - w.lc) * 8, c1 = c0 + P.ct * 8 < P.C ? c0 + P.ct * 8 : P.C, g0 = gn_div(c0, P.dm), g1 = gn_div(c1 - 1, P.dm);
+            const float* ref = P.part + (size_t)w.n * P.chunks * 2 * P.C;
+            gn_tile_groups<3>(P, w, g0, g1, [&](int g, int ch, int, const float2& m, double* v) __attribute__((always_inline)) {
+                gn_add_chunk(P, m, ch, (double)ref[2 * g * P.D], v);
+            }, [&](int g, const double* v) __attribute__((always_inline)) {
+                const float2 st = gn_group_stat(P, v, (double)ref[2 * g * P.D]);
+                stat[g - g0] = st;
+                if (w.chunk == 0) {
+                    P.mean[w.n * P.G + g] = st.x;
+                    P.rstd[w.n * P.G + g] = st.y;
+                }
+            });
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int g = gr.g[i] < g0 ? g0 : gr.g[i] > g1 ? g1 : gr.g[i];
+                k.mean[i] = stat[g - g0].x;
+                k.rstd[i] = stat[g - g0].y;
+            }
+            gn_param(P, w, k);
+        } else {
+            gn_coef(P, w, gr, k);
+        }
         af.set(k);
     }
     const bool silu = P.act == Y5M_ACT_SILU;
@@ -645,8 +712,8 @@ __global__ __launch_bounds__(GN_THREADS) void gn_param_grad_kernel(const GnParam
     }
 }
 
-template <int DT, int AL, int FMT, bool SILU>
-__device__ __forceinline__ void gn_bwd_rows(const GnParams& P, const GnPlace& w) {
+template <int DT, int AL, int FMT, bool SILU, bool INL>
+__device__ __forceinline__ void gn_bwd_rows(const GnParams& P, const GnPlace& w, const float2* lab, int g0) {
     typedef typename RowElem<DT>::T T;
     // dx = r gamma dt - r A - r B xhat = c1 dt + (c2 v + c3), v = xhat in f32, the kept value in 16 bits
     GnGrad<DT> grad;
@@ -658,7 +725,9 @@ __device__ __forceinline__ void gn_bwd_rows(const GnParams& P, const GnPlace& w)
         grad.set(k);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float2 ab = *reinterpret_cast<const float2*>(P.ab + (w.n * P.G + gr.g[i]) * 2);
+            // (channels behind the last: any of the tile's groups)
+            const int g = gr.g[i];
+            const float2 ab = INL ? lab[g - g0] : *reinterpret_cast<const float2*>(P.ab + (w.n * P.G + g) * 2);
             c1[i] = k.rstd[i] * k.gamma[i];
             c2[i] = -k.rstd[i] * ab.y;
             c3[i] = -k.rstd[i] * ab.x;
@@ -700,12 +769,39 @@ __device__ __forceinline__ void gn_bwd_rows(const GnParams& P, const GnPlace& w)
     }
 }
 
-template <int DT, int AL, int FMT>
+template <int DT, int AL, int FMT, bool INL>
 __global__ __launch_bounds__(GN_THREADS) void gn_bwd_apply_kernel(const GnParams P) {
     const GnPlace w = gn_place<true>(P, P.arpc);
-    if (w.n < 0 || !w.in) return;
-    if (P.act == Y5M_ACT_SILU) gn_bwd_rows<DT, AL, FMT, true>(P, w);
-    else gn_bwd_rows<DT, AL, FMT, false>(P, w);
+    if (w.n < 0) return;
+    const float2* lab = nullptr;
+    int g0 = 0;
+    if constexpr (INL) {
+        __shared__ float2 ab[GN_THREADS];
+        const int c0 = (w.piece - w.lc) * 8, c1 = c0 + P.ct * 8 < P.C ? c0 + P.ct * 8 : P.C, g1 = gn_div(c1 - 1, P.dm);
+        g0 = gn_div(c0, P.dm);
+        gn_tile_groups<2>(P, w, g0, g1, [&](int g, int, int d, const float2& m, double* v) __attribute__((always_inline)) {
+            const double ga = P.gamma ? (double)P.gamma[g * P.D + d] : 1.0;
+            v[0] += ga * (double)m.x;
+            v[1] += ga * (double)m.y;
+        }, [&](int g, const double* v) __attribute__((always_inline)) { ab[g - g0] = make_float2((float)(v[0] * P.inv_k), (float)(v[1] * P.inv_k)); });
+        if (w.chunk == 0) {                                        // the sample's channel sums, for the parameters' gradients
+            const float2* part = reinterpret_cast<const float2*>(P.part) + (size_t)w.n * P.chunks * P.C;
+            for (int c = c0 + (int)threadIdx.x; c < c1; c += GN_THREADS) {
+                double a = 0.0, b = 0.0;
+                for (int ch = 0; ch < P.chunks; ++ch) {
+                    const float2 m = part[(size_t)ch * P.C + c];
+                    a += (double)m.x;
+                    b += (double)m.y;
+                }
+                *reinterpret_cast<float2*>(P.nc + ((size_t)w.n * P.C + c) * 2) = make_float2((float)a, (float)b);
+            }
+        }
+        lab = ab;
+        __syncthreads();
+    }
+    if (!w.in) return;
+    if (P.act == Y5M_ACT_SILU) gn_bwd_rows<DT, AL, FMT, true, INL>(P, w, lab, g0);
+    else gn_bwd_rows<DT, AL, FMT, false, INL>(P, w, lab, g0);
 }
 
 // ---- held -------------------------------------------------------------------------------------------------------------------------
@@ -1032,7 +1128,7 @@ static void gn_geometry(GnParams& P, bool quads, int rows, int arows) {
 // scraps. Held against split, 20 x 20 x 768 bf16 in 32 groups: forward of 1 / 16 / 32 / 64 images 9 / 14 / 17 / 30 us against 14 / 18 / 23 / 32,
 // of 256 165 against 105; backward of 1 / 8 / 16 / 32 images 13 / 14 / 23 / 39 against 21 / 24 / 29 / 36. 16384 x 768 tokens (one row
 // each): forward 92 against 940. 16 rows a thread pay from 128 workgroups on: 64 / 128 / 256 of them (40 x 40, 96 and 192 channels) 13.4 /
-// 14.6 / 17.4 against 12.1 / 14.8 / 24.1; three of one channel per group, 7623 rows: 28.4 against 12.6.
+// 14.6 / 17.4 against 12.1 / 14.4 / 24.1; three of one channel per group, 7623 rows: 28.4 against 10.6.
 struct GnHeld { int threads, nr; };
 static GnHeld gn_held(GnParams& P, bool blocks, bool aligned, const int* nrs, int64_t most) {
     // whole groups, whole blocks or pieces; rows that start anywhere may be cut anywhere (at 8 channels or more: load_raw8)
@@ -1121,15 +1217,31 @@ static dim3 gn_grid(int64_t x, int64_t N) {
     } while (0)
 #define GN_LAUNCH2(K, x) hipLaunchKernelGGL(K, gn_grid((int64_t)(x), P.N), dim3(GN_THREADS), 0, st, P)
 
+// may the apply pass join the sums itself? At most 16 pairs a lane, outputs that stay in the caches (5 x 21 x 37 x 36 fp16 with the 8-bit
+// form, 12 groups: forward 12.9 -> 11.1 us, backward 18.5 -> 14.9; backward of 64 x 40 x 40 x 96 36 -> 30; at 64 pairs a lane one 80 x 80 x 96
+// map takes 12.6 and 26.3 where the launch of its own takes 11.3 and 16.4)
+static bool gn_inline(const GnParams& P) {
+    const int ng = (P.ct * 8 < P.C ? P.ct * 8 : P.C) / P.D + 2;    // groups that a tile touches, at most
+    if (ng > GN_THREADS) return false;
+    int k = 64;
+    while (ng * k > GN_THREADS && k > 1) k >>= 1;
+    return (int64_t)P.chunks * P.D <= 16ll * k;
+}
+
 template <int DT, int AL, int FMT> static int gn_fwd_split(GnParams& P, hipStream_t st) {
     gn_geometry(P, FMT != Y5M_KEEP_NONE, GN_ROWS, GN_APPLY_ROWS);
     GN_LAUNCH2((gn_stats_kernel<DT, AL>), P.chunks * P.tiles);
-    GN_JOINS(gn_stats_join_kernel);
-    if constexpr (AL > 0) {
-        if (rows_past_caches(P.N * P.S, P.C, DT)) GN_LAUNCH2((gn_apply_kernel<DT, 2, FMT>), P.achunks * P.tiles);
-        else GN_LAUNCH2((gn_apply_kernel<DT, 1, FMT>), P.achunks * P.tiles);
+    const bool past = rows_past_caches(P.N * P.S, P.C, DT);
+    if (!past && gn_inline(P)) {
+        GN_LAUNCH2((gn_apply_kernel<DT, AL, FMT, true>), P.achunks * P.tiles);
     } else {
-        GN_LAUNCH2((gn_apply_kernel<DT, AL, FMT>), P.achunks * P.tiles);
+        GN_JOINS(gn_stats_join_kernel);
+        if constexpr (AL > 0) {
+            if (past) GN_LAUNCH2((gn_apply_kernel<DT, 2, FMT, false>), P.achunks * P.tiles);
+            else GN_LAUNCH2((gn_apply_kernel<DT, AL, FMT, false>), P.achunks * P.tiles);
+        } else {
+            GN_LAUNCH2((gn_apply_kernel<DT, AL, FMT, false>), P.achunks * P.tiles);
+        }
     }
     Y5M_CHECK_LAUNCH("gn_apply_kernel");
     return Y5M_OK;
@@ -1193,12 +1305,17 @@ template <int DT, int AL, int FMT> static int gn_bwd(GnParams& P, hipStream_t st
     } else {
         gn_geometry(P, false, GN_ROWS, GN_APPLY_ROWS);
                 GN_LAUNCH2((gn_bwd_reduce_kernel<DT, AL, FMT>), P.chunks * P.tiles);
-        GN_JOINS(gn_bwd_join_kernel);
-        if constexpr (AL > 0) {
-            if (rows_past_caches(P.N * P.S, P.C, DT)) GN_LAUNCH2((gn_bwd_apply_kernel<DT, 2, FMT>), P.achunks * P.tiles);
-            else GN_LAUNCH2((gn_bwd_apply_kernel<DT, 1, FMT>), P.achunks * P.tiles);
+        const bool past = rows_past_caches(P.N * P.S, P.C, DT);
+        if (!past && gn_inline(P)) {
+            GN_LAUNCH2((gn_bwd_apply_kernel<DT, AL, FMT, true>), P.achunks * P.tiles);
         } else {
-            GN_LAUNCH2((gn_bwd_apply_kernel<DT, AL, FMT>), P.achunks * P.tiles);
+            GN_JOINS(gn_bwd_join_kernel);
+            if constexpr (AL > 0) {
+                if (past) GN_LAUNCH2((gn_bwd_apply_kernel<DT, 2, FMT, false>), P.achunks * P.tiles);
+                else GN_LAUNCH2((gn_bwd_apply_kernel<DT, AL, FMT, false>), P.achunks * P.tiles);
+            } else {
+                GN_LAUNCH2((gn_bwd_apply_kernel<DT, AL, FMT, false>), P.achunks * P.tiles);
+            }
         }
         Y5M_CHECK_LAUNCH("gn_bwd_apply_kernel");
     }
