@@ -29,8 +29,17 @@ _ACTS = {None: 0, "none": 0, "silu": 1}
 
 
 class GroupNormSaved:
-    """what a forward leaves for its backward: `kept` (the input tensor or an Act8), `mean`, `rstd` (N, groups) f32, the parameters"""
-    __slots__ = ("kept", "mean", "rstd", "groups", "act", "weight", "bias")
+    """what a forward leaves for its backward: `kept` (the input tensor or an Act8), `mean`, `rstd` (N, groups) f32 (one tensor, `stat`),
+    the parameters"""
+    __slots__ = ("kept", "stat", "groups", "act", "weight", "bias")
+
+    @property
+    def mean(self):
+        return self.stat[0]
+
+    @property
+    def rstd(self):
+        return self.stat[1]
 
 
 def _param(t, c, name, x):
@@ -87,7 +96,7 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="silu", keep
         return z, None
     sv = GroupNormSaved()
     sv.kept = a if a else x.detach()
-    sv.mean, sv.rstd, sv.groups, sv.act, sv.weight, sv.bias = stat[0], stat[1], groups, act, w, b
+    sv.stat, sv.groups, sv.act, sv.weight, sv.bias = stat, groups, act, w, b
     return z, sv
 
 
@@ -107,14 +116,15 @@ def group_norm_act_backward(dz, saved):
     with on_device_of(dz):
         dx = empty_rows(dz.shape, dz.dtype, dz.device)
         grads = torch.empty((2, c), dtype=torch.float32, device=dz.device)
+        mean, dgamma = saved.stat.data_ptr(), grads.data_ptr()
         wsb = L.y5m_gn_act_bwd_workspace_bytes(n, s, c, saved.groups)
         ws = torch.empty(wsb, dtype=torch.uint8, device=dz.device)
         _lib.check(L.y5m_gn_act_bwd(dz.data_ptr(), dn, dr, None if a else kept.data_ptr(), xn, xr, a.q.data_ptr() if a else None,
                                     a.q.shape[1] if a else 0, a.scale.data_ptr() if a else None, FORMATS[a.fmt] if a else 0, _ptr(saved.weight),
-                                    _ptr(saved.bias), saved.mean.data_ptr(), saved.rstd.data_ptr(), n, s, c, saved.groups, _ACTS[saved.act],
-                                    dx.data_ptr(), s * c, c, grads.data_ptr(), grads.data_ptr() + 4 * c, ws.data_ptr(), wsb, DTYPES[dz.dtype],
+                                    _ptr(saved.bias), mean, mean + 4 * n * saved.groups, n, s, c, saved.groups, _ACTS[saved.act],
+                                    dx.data_ptr(), s * c, c, dgamma, dgamma + 4 * c, ws.data_ptr(), wsb, DTYPES[dz.dtype],
                                     _lib.stream_ptr()), "y5m_gn_act_bwd")
-    return dx, grads[0], grads[1]
+    return (dx, *grads.unbind(0))
 
 
 class _GroupNormActFn(torch.autograd.Function):
@@ -122,10 +132,10 @@ class _GroupNormActFn(torch.autograd.Function):
     def forward(ctx, x, weight, bias, groups, eps, act, keep):
         z, sv = group_norm_act(x, groups, weight, bias, eps, act, keep)
         if isinstance(sv.kept, Act8):
-            ctx.save_for_backward(sv.kept.q, sv.kept.scale, sv.mean, sv.rstd, weight, bias)
+            ctx.save_for_backward(sv.kept.q, sv.kept.scale, sv.stat, weight, bias)
             ctx.act8 = (sv.kept.shape, sv.kept.dtype, sv.kept.fmt)
         else:
-            ctx.save_for_backward(x, None, sv.mean, sv.rstd, weight, bias)      # (autograd notices if x is overwritten meanwhile)
+            ctx.save_for_backward(x, None, sv.stat, weight, bias)      # (autograd notices if x is overwritten meanwhile)
             ctx.act8 = None
         ctx.meta = (groups, act)
         return z
@@ -133,13 +143,13 @@ class _GroupNormActFn(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dz):
-        k, scale, mean, rstd, weight, bias = ctx.saved_tensors
+        k, scale, stat, weight, bias = ctx.saved_tensors
         sv = GroupNormSaved()
         sv.kept = Act8(k, scale, *ctx.act8) if ctx.act8 else k
-        sv.mean, sv.rstd = mean, rstd
+        sv.stat = stat
         sv.groups, sv.act = ctx.meta
         c = sv.kept.shape[1]
-        sv.weight, sv.bias = _param(weight, c, "weight", mean), _param(bias, c, "bias", mean)
+        sv.weight, sv.bias = _param(weight, c, "weight", stat), _param(bias, c, "bias", stat)
         try:
             rows_of(dz, "dz")
         except Y5MError:                                       # autograd hands over what the consumer produced: lay it out
