@@ -576,3 +576,54 @@ def test_a_kept_form_needs_group_norm():
     from yolov5m_amd.model import CBL
     with pytest.raises(Y5MError, match="norm_groups"):
         CBL(8, 8, 1, 1, 0, keep="int8")
+
+
+SPLIT = [((5, 36, 21, 37), 12, "fp16"), ((3, 29, 121, 63), 29, "bf16"), ((1, 96, 80, 80), 32, "bf16"), ((2, 768, 30, 30), 1, "bf16"), ((1, 1386, 31, 5), 2, "f32"),
+         ((1, 2112, 12, 11), 3, "bf16"), ((9, 64, 40, 40), 64, "f32")]
+
+
+@pytest.mark.parametrize("keep", ["x", "int8"])
+@pytest.mark.parametrize("case", SPLIT)
+def test_few_and_many_sums_to_join(case, keep):
+    """maps too long for one workgroup: sums joined by the apply pass, by 256 and by 1024 threads a group, groups across column tiles"""
+    from yolov5m_amd.group_norm import group_norm_act, group_norm_act_backward
+    shape, groups, dtype = case
+    if DEV != "cuda" and shape[0] * shape[1] * shape[2] * shape[3] > 10 ** 6:
+        pytest.skip("long on the executor")
+    x, dz = _rows(shape, dtype, 100, offset=0.5), _rows(shape, dtype, 101, scale=0.1)
+    ga, be = _params(shape[1], 102)
+    kept = None if keep == "x" else stored_values(x, keep)[0]
+    ref = Exact(x, groups, ga, be, 1e-3, "silu", kept, dz)
+    z, saved = group_norm_act(x, groups, ga, be, eps=1e-3, keep=keep)
+    ref.check(z, "z")
+    assert ((saved.mean.cpu().double().flatten() - ref.mean).abs() <= 64 * U * (ref.mean.abs() + 1 / ref.rstd)).all()
+    assert ((saved.rstd.cpu().double().flatten() - ref.rstd).abs() <= 64 * U * ref.rstd).all()
+    for got, what in zip(group_norm_act_backward(dz, saved), ("dx", "dgamma", "dbeta")):
+        ref.check(got, what)
+
+
+@pytest.mark.parametrize("case", SPLIT)
+def test_captured_split_forms(case):
+    """captured, replayed with new inputs and eager calls between the replays: equal to the eager result"""
+    if DEV != "cuda":
+        pytest.skip("graphs")
+    from yolov5m_amd.group_norm import group_norm_act, group_norm_act_backward
+    shape, groups, dtype = case
+    ga, be = _params(shape[1], 103)
+
+    def step(x, dz):
+        z, saved = group_norm_act(x, groups, ga, be, keep="e4m3")
+        return (z, *group_norm_act_backward(dz, saved))
+    x, dz = _rows(shape, dtype, 104), _rows(shape, dtype, 105)
+    step(x, dz)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step(x, dz)
+    for seed in (106, 107, 108):
+        x.copy_(_rows(shape, dtype, seed))
+        dz.copy_(_rows(shape, dtype, seed + 50))
+        g.replay()
+        want = step(x, dz)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, out)), seed

@@ -303,7 +303,8 @@ template <int NV, typename V, typename F> __device__ __forceinline__ void gn_til
     while ((g1 - g0 + 1) * k > GN_THREADS && k > 1) k >>= 1;
     const int sub = threadIdx.x & (k - 1), pairs = P.chunks * P.D;
     const float2* part = reinterpret_cast<const float2*>(P.part) + (size_t)w.n * P.chunks * P.C;
-    for (int g = g0 + (int)threadIdx.x / k; g <= g1; g += GN_THREADS / k) {
+    for (int b = g0; b <= g1; b += GN_THREADS / k) {               // (every lane runs the same trips: they meet in the shuffles)
+        const int at = b + (int)threadIdx.x / k, g = at < g1 ? at : g1;
         double v[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i) v[i] = 0.0;
@@ -324,7 +325,7 @@ template <int NV, typename V, typename F> __device__ __forceinline__ void gn_til
         for (int o = k >> 1; o > 0; o >>= 1)
 #pragma unroll
             for (int i = 0; i < NV; ++i) v[i] += gn_shfl_xor(v[i], o);
-        if (sub == 0) f(g, v);
+        if (sub == 0 && at <= g1) f(g, v);
     }
 }
 
