@@ -627,3 +627,26 @@ def test_captured_split_forms(case):
         want = step(x, dz)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(want, out)), seed
+
+
+# (samples, channels, rows, groups): long enough for the split form, one chunk with many rows side by side where there are few channels
+OUTLIER = [((1, 8, 25600), 1), ((1, 8, 5000), 4), ((1, 16, 25600), 4), ((1, 48, 25600), 6), ((1, 768, 2600), 1)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("case", OUTLIER)
+def test_an_outlier_first_row_at_every_width(case, dtype):
+    """a first row of 1000 before N(0, 1): whatever shares a chunk with it, the statistics and outputs stay within the bounds of a computation
+    that sums about the mean (rstd: the f64 sums leave the rounding to f32, two u)"""
+    from yolov5m_amd.group_norm import group_norm_act
+    shape, groups = case
+    if DEV != "cuda" and shape[1] > 100:
+        pytest.skip("long on the executor")
+    x = torch.randn((shape[0], shape[2], shape[1]), generator=torch.Generator().manual_seed(110))
+    x[:, 0] = 1000.0
+    x = x.to(DT[dtype]).movedim(-1, 1).to(DEV)
+    ref = Exact(x, groups, None, None, 1e-5, None)
+    z, saved = group_norm_act(x, groups, act=None, keep="x")
+    ref.check(z, "z")
+    assert ((saved.rstd.cpu().double().flatten() - ref.rstd).abs() <= 8 * U * ref.rstd).all()
+    assert ((saved.mean.cpu().double().flatten() - ref.mean).abs() <= 8 * U * (ref.mean.abs() + 1 / ref.rstd)).all()

@@ -98,22 +98,28 @@ __device__ __forceinline__ GnGroups gn_groups(const GnParams& P, int c) {
 
 // sums over the RP rows that a workgroup holds side by side: v[16] = two sums of 8 channels per thread. f(channel, sum, sum) for each
 // channel, one thread per channel
-template <typename F>
-__device__ __forceinline__ void gn_join_rows(const float* v, float* red, const GnPlace& w, int ct, int RP, int C, F f) {
+template <typename A, typename F>
+__device__ __forceinline__ void gn_join_rows(const A* v, A* red, const GnPlace& w, int ct, int RP, int C, F f) {
+    typedef A V __attribute__((ext_vector_type(16 / sizeof(A))));
+    constexpr int NV = 16 / (int)sizeof(A);
     const int wd = ct * 8, c0 = (w.piece - w.lc) * 8;
-    float* red2 = red + GN_THREADS * 8;
+    A* red2 = red + GN_THREADS * 8;
     if (w.in) {
-        float4 *d = reinterpret_cast<float4*>(red + w.lr * wd + w.lc * 8), *d2 = reinterpret_cast<float4*>(red2 + w.lr * wd + w.lc * 8);
-        d[0] = make_float4(v[0], v[1], v[2], v[3]);
-        d[1] = make_float4(v[4], v[5], v[6], v[7]);
-        d2[0] = make_float4(v[8], v[9], v[10], v[11]);
-        d2[1] = make_float4(v[12], v[13], v[14], v[15]);
+        V *d = reinterpret_cast<V*>(red + w.lr * wd + w.lc * 8), *d2 = reinterpret_cast<V*>(red2 + w.lr * wd + w.lc * 8);
+#pragma unroll
+        for (int i = 0; i < 8 / NV; ++i) {
+            V t, t2;
+#pragma unroll
+            for (int k = 0; k < NV; ++k) { t[k] = v[i * NV + k]; t2[k] = v[8 + i * NV + k]; }
+            d[i] = t;
+            d2[i] = t2;
+        }
     }
     __syncthreads();
     const int parts = GN_THREADS / wd;
     if (parts < 2) {
         for (int j = threadIdx.x; j < wd; j += GN_THREADS) {
-            float a = 0.f, b = 0.f;
+            A a = 0, b = 0;
             for (int r = 0; r < RP; ++r) {
                 a += red[r * wd + j];
                 b += red2[r * wd + j];
@@ -124,11 +130,11 @@ __device__ __forceinline__ void gn_join_rows(const float* v, float* red, const G
     }
     // spare threads take every parts-th row; their sums meet in LDS
     const int part = (int)threadIdx.x / wd, j = (int)threadIdx.x - part * wd;
-    float a = 0.f, b = 0.f;
+    A a = 0, b = 0;
     if (part < parts) {
         int r = part;
         for (; r + 3 * parts < RP; r += 4 * parts) {
-            float u[4], v4[4];
+            A u[4], v4[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) { u[k] = red[(r + k * parts) * wd + j]; v4[k] = red2[(r + k * parts) * wd + j]; }
 #pragma unroll
@@ -157,34 +163,33 @@ __device__ __forceinline__ void gn_join_rows(const float* v, float* red, const G
 __device__ __forceinline__ float2* gn_part(const GnParams& P, const GnPlace& w, int c) { return reinterpret_cast<float2*>(P.part) + ((size_t)w.n * P.chunks + w.chunk) * P.C + c; }
 
 // ---- forward, split ---------------------------------------------------------------------------------------------------------------
-// Squares are summed about the chunk's first row: a chunk's mean and M2 = sum (x - p)^2 - (sum (x - p))^2 / R then cancel by at most a
-// factor R (a few hundred), even if that row is an outlier; chunks are joined by the pairwise formula.
+// Values and squares are summed in f64, where the square of an f32 is exact: M2 = sum x^2 - (sum x)^2 / R loses mean^2 / var of 2^-53, whichever
+// row comes first and however many share a chunk. (In f32 about the chunk's first row an outlier there cost up to R of 2^-24, R = 4096 rows at 8
+// channels. The f64 additions run at the rate of scalar f32 ones and hide behind the loads.) Chunks are joined by the pairwise formula.
 template <int DT, int AL>
 __global__ __launch_bounds__(GN_THREADS) void gn_stats_kernel(const GnParams P) {
     typedef typename RowElem<DT>::T T;
-    __shared__ __attribute__((aligned(16))) float red[GN_THREADS * 16];
+    __shared__ __attribute__((aligned(16))) double red[GN_THREADS * 16];
     const GnPlace w = gn_place<false>(P, P.rpc);
     if (w.n >= P.N) return;
-    float a[16], pv[8];
+    double a[16];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) a[k] = 0.f;
-    const T* b = static_cast<const T*>(P.x) + w.n * P.xn + w.c;
+    for (int k = 0; k < 16; ++k) a[k] = 0.0;
     if (w.in) {
-        load8<DT, AL>(b + (int64_t)w.r0 * P.xr, w.nv, pv);
         auto add = [&](const Raw8<DT>& raw) __attribute__((always_inline)) {
             float v[8];
             unpack8<DT>(raw, v);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const float d = v[k] - pv[k];
+                const double d = (double)v[k];
                 a[k] += d;
-                a[8 + k] = fmaf(d, d, a[8 + k]);
+                a[8 + k] = fma(d, d, a[8 + k]);
             }
         };
         constexpr int U = 4;                                       // rows in flight (8: five waves per SIMD instead of eight, no faster)
         const int64_t step = (int64_t)P.RP * P.xr;
         int r = w.r0 + w.lr;
-        const T* p = b + (int64_t)r * P.xr;
+        const T* p = static_cast<const T*>(P.x) + w.n * P.xn + w.c + (int64_t)r * P.xr;
         for (; r + (U - 1) * P.RP < w.r1; r += U * P.RP) {
             Raw8<DT> raw[U];
 #pragma unroll
@@ -200,15 +205,11 @@ __global__ __launch_bounds__(GN_THREADS) void gn_stats_kernel(const GnParams P) 
             p += step;
         }
     }
-    // channel sums about the first row -> the chunk's mean and M2
-    const float R = (float)(w.r1 - w.r0);
-    const T* first = static_cast<const T*>(P.x) + w.n * P.xn + (int64_t)w.r0 * P.xr;
-    gn_join_rows(a, red, w, P.ct, P.RP, P.C, [&](int c, float s1, float s2) __attribute__((always_inline)) {
-        float pv;
-        if constexpr (DT == Y5M_F32) pv = first[c];
-        else if constexpr (DT == Y5M_BF16) pv = bf16_to_f32(first[c]);
-        else pv = f16_to_f32(first[c]);
-        *gn_part(P, w, c) = make_float2(pv + s1 / R, s2 - s1 * s1 / R);
+    // -> the chunk's mean and M2
+    const double R = (double)(w.r1 - w.r0), inv = 1.0 / R;
+    gn_join_rows(a, red, w, P.ct, P.RP, P.C, [&](int c, double s1, double s2) __attribute__((always_inline)) {
+        const double m = s1 * inv, m2 = fma(-s1, m, s2);
+        *gn_part(P, w, c) = make_float2((float)m, (float)(m2 < 0.0 ? 0.0 : m2));          // (a NaN stays)
     });
 }
 
