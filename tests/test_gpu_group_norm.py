@@ -650,3 +650,21 @@ def test_an_outlier_first_row_at_every_width(case, dtype):
     ref.check(z, "z")
     assert ((saved.rstd.cpu().double().flatten() - ref.rstd).abs() <= 8 * U * ref.rstd).all()
     assert ((saved.mean.cpu().double().flatten() - ref.mean).abs() <= 8 * U * (ref.mean.abs() + 1 / ref.rstd)).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [1, 50, 100, 5000])
+def test_statistics_over_the_whole_range_of_the_type(rows, dtype):
+    """finite inputs whose squares leave f32: a first row of 1e17 / 1e18 / 1e30 before N(0, 1), maps around 1e18 and 3e37, and one of 1e-25 (its
+    squares are below f32, as its eps is). Held and split form alike, within the bounds of ordinary inputs"""
+    from yolov5m_amd.group_norm import group_norm_act
+    for first, scale, offset, eps in ((1e17, 1.0, 0.0, 1e-5), (1e18, 1.0, 0.0, 1e-5), (1e30, 1.0, 0.0, 1e-5), (None, 1e17, 1e18, 1e-5), (None, 3e37, 0.0, 1e-5),
+                                      (None, 1e-25, 0.0, 1e-37)):
+        x = torch.randn((2, rows, 16), generator=torch.Generator().manual_seed(111)).clamp(-4, 4) * scale + offset
+        if first is not None:
+            x[:, 0] = first
+        x = x.to(DT[dtype]).movedim(-1, 1).to(DEV)
+        ref = Exact(x, 4, None, None, eps, None)
+        z, saved = group_norm_act(x, 4, act=None, eps=eps, keep="x")
+        assert ((saved.rstd.cpu().double().flatten() - ref.rstd).abs() <= 64 * U * ref.rstd).all(), (first, scale)
+        ref.check(z, "z")

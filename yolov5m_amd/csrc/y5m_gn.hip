@@ -30,7 +30,7 @@ struct GnParams {
     const float *gamma, *beta;     // null: 1, 0
     float *mean, *rstd;            // [N][G]
     uint8_t *q, *scale;            // 8-bit form
-    float* part;                   // split: [N][chunks][C][2] channel sums: mean and M2 of the chunk; backward: sum dt, sum dt xhat
+    float* part;                   // split: [N][chunks][C][2] of a channel in a chunk: mean and deviation; backward: sum dt, sum dt xhat
     float* nc;                     // backward: [N][C][2] channel sums
     float* ab;                     // backward, split: [N][G][2] A, B
     float *dgamma, *dbeta;
@@ -165,7 +165,8 @@ __device__ __forceinline__ float2* gn_part(const GnParams& P, const GnPlace& w, 
 // ---- forward, split ---------------------------------------------------------------------------------------------------------------
 // Values and squares are summed in f64, where the square of an f32 is exact: M2 = sum x^2 - (sum x)^2 / R loses mean^2 / var of 2^-53, whichever
 // row comes first and however many share a chunk. (In f32 about the chunk's first row an outlier there cost up to R of 2^-24, R = 4096 rows at 8
-// channels. The f64 additions run at the rate of scalar f32 ones and hide behind the loads.) Chunks are joined by the pairwise formula.
+// channels. The f64 additions run at the rate of scalar f32 ones and hide behind the loads.) A chunk leaves its mean and sqrt(M2 / R),
+// which f32 holds for every input, where M2 overflows from deviations of 2^60 on. Chunks are joined by the pairwise formula, in f64.
 template <int DT, int AL>
 __global__ __launch_bounds__(GN_THREADS) void gn_stats_kernel(const GnParams P) {
     typedef typename RowElem<DT>::T T;
@@ -205,11 +206,11 @@ __global__ __launch_bounds__(GN_THREADS) void gn_stats_kernel(const GnParams P) 
             p += step;
         }
     }
-    // -> the chunk's mean and M2
+    // -> the chunk's mean and deviation
     const double R = (double)(w.r1 - w.r0), inv = 1.0 / R;
     gn_join_rows(a, red, w, P.ct, P.RP, P.C, [&](int c, double s1, double s2) __attribute__((always_inline)) {
         const double m = s1 * inv, m2 = fma(-s1, m, s2);
-        *gn_part(P, w, c) = make_float2((float)m, (float)(m2 < 0.0 ? 0.0 : m2));          // (a NaN stays)
+        *gn_part(P, w, c) = make_float2((float)m, (float)sqrt(m2 < 0.0 ? 0.0 : m2 * inv));          // (a NaN stays)
     });
 }
 
@@ -252,18 +253,23 @@ template <int T> __device__ __forceinline__ GnWalk gn_walk(int D) {
     return k;
 }
 
+// 1 / sqrt(v): in f32 where v is well inside its range, which is where the other way's time would be noticed
+__device__ __forceinline__ float gn_rsqrt(double v) {
+    const float f = (float)v;
+    return f > 1e-30f && f < 1e30f ? 1.0f / sqrtf(f) : (float)(1.0 / sqrt(v));
+}
 // a group's mean and rstd from its chunks' sums about ref: sum R (m - ref), sum R (m - ref)^2, sum M2
 __device__ __forceinline__ float2 gn_group_stat(const GnParams& P, const double* v, double ref) {
     const double off = v[0] * P.inv_k;
     double var = (v[2] + v[1]) * P.inv_k - off * off;
     if (!(var > 0.0) && var == var) var = 0.0;                     // (a NaN stays)
-    return make_float2((float)(ref + off), 1.0f / sqrtf((float)(var + (double)P.eps)));
+    return make_float2((float)(ref + off), gn_rsqrt(var + (double)P.eps));
 }
 __device__ __forceinline__ void gn_add_chunk(const GnParams& P, const float2& m, int ch, double ref, double* v) {
     const double R = (double)(ch + 1 < P.chunks ? P.rpc : P.S - ch * P.rpc), e = (double)m.x - ref;
     v[0] += R * e;
     v[1] += R * e * e;
-    v[2] += (double)m.y;
+    v[2] += R * (double)m.y * (double)m.y;
 }
 
 template <int T> __global__ __launch_bounds__(T) void gn_stats_join_kernel(const GnParams P) {
@@ -808,7 +814,7 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_apply_kernel(const GnParams
 
 // ---- held -------------------------------------------------------------------------------------------------------------------------
 // A workgroup of up to 512 threads (256 registers each) holds a slice of `sc` channels (whole groups; whole 32-channel blocks where the 8-bit form is
-// written) of one sample: NR row pieces per thread, RP rows side by side, two plain passes over registers for mean and variance.
+// written) of one sample: NR row pieces per thread, RP rows side by side.
 // Slices of a sample follow each other on one XCD (the hardware deals workgroups round the 8 XCDs): a row's cache lines, which several
 // slices share, are fetched once.
 #define GN_HELD_THREADS 512
@@ -828,24 +834,30 @@ __device__ __forceinline__ GnSlice gn_slice(const GnParams& P) {
     w.in = w.lr < P.RP && w.nv > 0;
     return w;
 }
-// NS sums of 8 channels per thread -> tot[which][channel of the slice] in LDS. red: NS * 8 * threads floats, sub: threads floats,
-// tot: NS * sc floats
-template <int NS> __device__ __forceinline__ void gn_slice_sums(const GnParams& P, const GnSlice& w, const float* v, float* red, float* sub, float* tot) {
+// NS sums of 8 channels per thread -> tot[which][channel of the slice] in LDS. red: NS * 8 * threads values, sub: threads, tot: NS * sc
+template <int NS, typename A> __device__ __forceinline__ void gn_slice_sums(const GnParams& P, const GnSlice& w, const A* v, A* red, A* sub, A* tot) {
+    typedef A V __attribute__((ext_vector_type(16 / sizeof(A))));
+    constexpr int NV = 16 / (int)sizeof(A);
     const int T = (int)blockDim.x, wd = P.ct * 8, cols = NS * wd;
     __syncthreads();
     if (w.in) {
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-            float4* d = reinterpret_cast<float4*>(red + w.lr * cols + s * wd + w.lc * 8);
-            d[0] = make_float4(v[s * 8], v[s * 8 + 1], v[s * 8 + 2], v[s * 8 + 3]);
-            d[1] = make_float4(v[s * 8 + 4], v[s * 8 + 5], v[s * 8 + 6], v[s * 8 + 7]);
+            V* d = reinterpret_cast<V*>(red + w.lr * cols + s * wd + w.lc * 8);
+#pragma unroll
+            for (int i = 0; i < 8 / NV; ++i) {
+                V t;
+#pragma unroll
+                for (int k = 0; k < NV; ++k) t[k] = v[s * 8 + i * NV + k];
+                d[i] = t;
+            }
         }
     }
     __syncthreads();
     const int rows = P.RP < P.S ? P.RP : P.S, parts = T / cols > 0 ? T / cols : 1;
     for (int j = threadIdx.x; j < cols * parts; j += T) {
         const int part = j / cols, c = j - part * cols;
-        float a = 0.f;
+        A a = 0;
         for (int r = part; r < rows; r += parts) a += red[r * cols + c];
         if (parts > 1) sub[j] = a;
         else tot[c] = a;
@@ -853,7 +865,7 @@ template <int NS> __device__ __forceinline__ void gn_slice_sums(const GnParams& 
     __syncthreads();
     if (parts > 1) {
         for (int c = threadIdx.x; c < cols; c += T) {
-            float a = 0.f;
+            A a = 0;
             for (int p = 0; p < parts; ++p) a += sub[p * cols + c];
             tot[c] = a;
         }
@@ -891,8 +903,9 @@ template <int NV, typename V, typename F> __device__ __forceinline__ void gn_sli
 template <int DT, int AL, int FMT, int NR>
 __global__ __launch_bounds__(GN_HELD_THREADS) void gn_held_kernel(const GnParams P) {
     typedef typename RowElem<DT>::T T;
-    extern __shared__ __attribute__((aligned(16))) float lds[];
-    float *red = lds, *sub = red + 16 * blockDim.x, *tot = sub + blockDim.x, *gm = tot + P.ct * 16, *gr = gm + P.ct * 8;
+    extern __shared__ __attribute__((aligned(16))) double lds64[];
+    double *red = lds64, *sub = red + 8 * blockDim.x, *tot = sub + blockDim.x;
+    float *gm = reinterpret_cast<float*>(tot + P.ct * 16), *gr = gm + P.ct * 8;
     const GnSlice w = gn_slice(P);
     const T* b = static_cast<const T*>(P.x) + w.n * P.xn + (w.in ? w.c : w.c0);
     const int nvl = w.in ? w.nv : w.nc, lr = w.lr < P.RP ? w.lr : 0;
@@ -902,28 +915,10 @@ __global__ __launch_bounds__(GN_HELD_THREADS) void gn_held_kernel(const GnParams
         const int r = lr + i * P.RP;
         raw[i] = load_raw8<DT, AL>(b + (int64_t)(r < P.S ? r : P.S - 1) * P.xr, nvl);
     }
-    float a[16], m[8];
+    // (sums and squares in f64: gn_stats_kernel says why)
+    double a[16];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) a[k] = 0.f;
-#pragma unroll
-    for (int i = 0; i < NR; ++i) {
-        const bool ok = lr + i * P.RP < P.S;
-        float v[8];
-        unpack8<DT>(raw[i], v);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) a[k] += ok ? v[k] : 0.f;
-    }
-    gn_slice_sums<1>(P, w, a, red, sub, tot);
-    gn_slice_groups<1>(P, w, [&](int c, int) __attribute__((always_inline)) { return (double)tot[c]; },
-                       [&](int g, const double* s) __attribute__((always_inline)) { gm[g] = (float)(s[0] * P.inv_k); });
-    __syncthreads();
-    const GnGroups gi = gn_groups(P, w.in ? w.lc * 8 : 0);         // (groups of the slice)
-    const int glast = gn_div(w.nc, P.dm) - 1;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) m[k] = gm[gi.g[k] < glast ? gi.g[k] : glast];
-#pragma unroll
-    for (int k = 0; k < 16; ++k) a[k] = 0.f;
-    // about that mean: the squares, and the rest of the mean (what the first sum's rounding lost)
+    for (int k = 0; k < 16; ++k) a[k] = 0.0;
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
         const bool ok = lr + i * P.RP < P.S;
@@ -931,16 +926,17 @@ __global__ __launch_bounds__(GN_HELD_THREADS) void gn_held_kernel(const GnParams
         unpack8<DT>(raw[i], v);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const float d = ok ? v[k] - m[k] : 0.f;
+            const double d = (double)(ok ? v[k] : 0.f);
             a[k] += d;
-            a[8 + k] = fmaf(d, d, a[8 + k]);
+            a[8 + k] = fma(d, d, a[8 + k]);
         }
     }
-    gn_slice_sums<2>(P, w, a, red, sub, tot);
     const int wd = P.ct * 8;
-    gn_slice_groups<2>(P, w, [&](int c, int i) __attribute__((always_inline)) { return (double)tot[i * wd + c]; }, [&](int g, const double* s) __attribute__((always_inline)) {
-        const double off = s[0] * P.inv_k, var = s[1] * P.inv_k - off * off;
-        const float mean = (float)((double)gm[g] + off), rs = 1.0f / sqrtf((float)((var > 0.0 || var != var ? var : 0.0) + (double)P.eps));
+    gn_slice_sums<1>(P, w, a, red, sub, tot);
+    gn_slice_sums<1>(P, w, a + 8, red, sub, tot + wd);
+    gn_slice_groups<2>(P, w, [&](int c, int i) __attribute__((always_inline)) { return tot[i * wd + c]; }, [&](int g, const double* s) __attribute__((always_inline)) {
+        const double md = s[0] * P.inv_k, var = fma(-md, md, s[1] * P.inv_k);
+        const float mean = (float)md, rs = gn_rsqrt((var < 0.0 ? 0.0 : var) + (double)P.eps);          // (a NaN stays)
         gm[g] = mean;
         gr[g] = rs;
         const int64_t ng = w.n * P.G + gn_div(w.c0, P.dm) + g;
@@ -948,15 +944,16 @@ __global__ __launch_bounds__(GN_HELD_THREADS) void gn_held_kernel(const GnParams
         P.rstd[ng] = rs;
     });
     __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 8; ++k) m[k] = gm[gi.g[k] < glast ? gi.g[k] : glast];
+    const GnGroups gi = gn_groups(P, w.in ? w.lc * 8 : 0);         // (groups of the slice)
+    const int glast = gn_div(w.nc, P.dm) - 1;
     GnAffine<DT> af;
     {
         GnCoef k;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            k.mean[i] = m[i];
-            k.rstd[i] = gr[gi.g[i] < glast ? gi.g[i] : glast];
+            const int g = gi.g[i] < glast ? gi.g[i] : glast;
+            k.mean[i] = gm[g];
+            k.rstd[i] = gr[g];
             const int c = w.in && i < w.nv ? w.c + i : w.c0;
             k.gamma[i] = P.gamma ? P.gamma[c] : 1.0f;
             k.beta[i] = P.beta ? P.beta[c] : 0.0f;
@@ -1257,7 +1254,7 @@ template <int DT, int AL, int FMT> static int gn_fwd_split(GnParams& P, hipStrea
 template <int DT, int AL, int FMT> static int gn_fwd(GnParams& P, hipStream_t st) {
     const GnHeld h = gn_held(P, FMT != Y5M_KEEP_NONE, AL > 0, GN_FWD_ROWS, GN_HELD_FWD);
     if (h.nr == 0) return gn_fwd_split<DT, AL, FMT>(P, st);
-    const int lds = (17 * h.threads + 4 * P.ct * 8) * (int)sizeof(float);
+    const int lds = (18 * h.threads + 6 * P.ct * 8) * (int)sizeof(float);
     if (h.nr == 4) GN_HELD_LAUNCH((gn_held_kernel<DT, AL, FMT, 4>), lds);
     else GN_HELD_LAUNCH((gn_held_kernel<DT, AL, FMT, 16>), lds);
     Y5M_CHECK_LAUNCH("gn_held_kernel");
