@@ -312,3 +312,26 @@ def test_wgrad_of_few_and_odd_channels(cout, dtype):
         dv = dy.cpu().double().movedim(1, -1).reshape(-1, cout)
         assert ((dw.cpu().double() - dv.t() @ xv).abs() <= 96 * U * (dv.abs().t() @ xv.abs())).all()
         assert ((db.cpu().double() - dv.sum(0)).abs() <= 160 * U * dv.abs().sum(0)).all()
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "fp16"])
+@pytest.mark.parametrize("case", [(16, 24, 9), (96, 136, 40), (20, 33, 40), (72, 3, 40)])
+def test_wgrad_of_the_largest_kept_values(case, dtype, fmt):
+    """blocks up to the largest magnitude that is held (a scale of 2^121 in int8), rows of ordinary and of tiny blocks beside them: the products
+    are those of the values read back. At most 40 rows: two instructions of 32 products, 34 roundings"""
+    from yolov5m_amd.act8 import act8_load, act8_store, act8_wgrad
+    c, cout, s = case
+    x = rows_tensor((1, c, s), "f32", 120)
+    big = torch.finfo(torch.float32).max
+    x[0, :, 1] = big
+    x[0, ::3, 1] = -big / 3
+    x[0, :, 2] = big / 2.0 ** 0.75 * torch.linspace(-1, 1, c).to(DEV)
+    x[0, :, 4] = 2.0 ** -110
+    dy = rows_tensor((1, cout, s), dtype, 121)
+    dy[0, :, 1:3] = dy[0, :, 1:3] * 2.0 ** -8
+    kept = act8_store(x, fmt)
+    dw, _ = act8_wgrad(dy, kept)
+    xv, dv = act8_load(kept).cpu().double()[0], dy.cpu().double()[0]
+    assert torch.isfinite(xv).all() and float(xv.abs().max()) > 0.9 * big
+    assert ((dw.cpu().double() - dv @ xv.t()).abs() <= 34 * U * (dv.abs() @ xv.abs().t())).all()

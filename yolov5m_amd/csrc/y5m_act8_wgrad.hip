@@ -180,10 +180,8 @@ template <int FMT> __device__ __forceinline__ unsigned aw_decode2(unsigned w, fl
     if constexpr (FMT == Y5M_KEEP_E4M3) {
         return __builtin_bit_cast(unsigned, h ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false));
     } else {
-        // bytes + 128 convert in one instruction each; (b - 128) * scale as one fma, exact
-        const unsigned u = w ^ 0x80808080u;
-        const float off = -128.0f * scale;
-        return f32x2_to_bf16x2(fmaf((float)((u >> (16 * h)) & 0xffu), scale, off), fmaf((float)((u >> (16 * h + 8)) & 0xffu), scale, off));
+        // (a signed byte converts in one instruction; as (b + 128) * scale - 128 * scale in one fma the offset left f32 at the largest scale)
+        return f32x2_to_bf16x2((float)(int8_t)(w >> (16 * h)) * scale, (float)(int8_t)(w >> (16 * h + 8)) * scale);
     }
 }
 
