@@ -285,6 +285,11 @@ static inline float __builtin_amdgcn_rcpf(float x) {
 }
 static inline float __builtin_amdgcn_rsqf(float x) { return 1.0f / sqrtf(x); }
 static inline float __builtin_amdgcn_exp2f(float x) { return exp2f(x); }
+// v_med3_f32: with a NaN among them the smallest of the others
+static inline float __builtin_amdgcn_fmed3f(float a, float b, float c) {
+    if (a != a || b != b || c != c) return fminf(fminf(a, b), c);
+    return fmaxf(fminf(a, b), fminf(fmaxf(a, b), c));
+}
 static inline const void* __builtin_amdgcn_kernarg_segment_ptr() { return emu::g.kernarg; }
 
 // OCP fp8 e4m3 (bias 7, largest 448, subnormals in steps of 2^-9, 0x7f / 0xff NaN): round to nearest even; beyond 448 + half a step NaN

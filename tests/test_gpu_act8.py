@@ -335,3 +335,36 @@ def test_wgrad_of_the_largest_kept_values(case, dtype, fmt):
     xv, dv = act8_load(kept).cpu().double()[0], dy.cpu().double()[0]
     assert torch.isfinite(xv).all() and float(xv.abs().max()) > 0.9 * big
     assert ((dw.cpu().double() - dv @ xv.t()).abs() <= 34 * U * (dv.abs() @ xv.abs().t())).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "fp16"])
+@pytest.mark.parametrize("case", [(40, 64, 70), (40, 65, 70), (96, 3, 70), (160, 136, 70)])
+def test_wgrad_of_large_and_infinite_gradients(case, dtype):
+    """dy with the largest finite values of its type, infinities and a NaN, over all ways in which rows are read: a product that is finite in 64
+    bits is finite and right (70 rows: three instructions of 32 products, 36 roundings), an infinity gives the signed infinity, or NaN against
+    a zero or another sign, as in 64 bits; db alike"""
+    from yolov5m_amd.act8 import act8_load, act8_store, act8_wgrad
+    c, cout, s = case
+    x = rows_tensor((1, c, s), "f32", 122) * 2.0 ** -12
+    dy = rows_tensor((1, cout, s), dtype, 123)
+    big = torch.finfo(DT[dtype]).max
+    dy[0, 0, 5], dy[0, 0, 40] = big, -big
+    dy[0, 1, 33] = big * (1 - 2.0 ** -9)
+    inf = float("inf")
+    dy[0, 2, 7] = inf
+    x[0, 1, 7] = 0.0
+    if cout > 8:
+        dy[0, 3, 9] = -inf
+        dy[0, 4, 9], dy[0, 4, 69] = inf, -inf
+        dy[0, 5, 0] = float("nan")
+        dy[0, cout - 1, 69] = -big
+    kept = act8_store(x, "e4m3")
+    dw, db = act8_wgrad(dy, kept, bias=True)
+    xv, dv = act8_load(kept).cpu().double()[0], dy.cpu().double()[0]
+    want, mag, sums = dv @ xv.t(), dv.abs() @ xv.abs().t(), dv.sum(1)
+    assert not torch.isfinite(want[2]).any() and torch.isfinite(want[:2]).all()
+    for got, ref, tol in ((dw, want, 36 * U * mag), (db, sums, 20 * U * dv.abs().sum(1))):
+        got, fin = got.cpu().double(), torch.isfinite(ref)
+        assert same(got[~fin], ref[~fin])
+        ok = fin & (ref.abs() + tol < 0.9 * torch.finfo(torch.float32).max) & (tol < big)
+        assert ((got - ref).abs() <= tol)[ok].all()
