@@ -368,3 +368,20 @@ def test_wgrad_of_large_and_infinite_gradients(case, dtype):
         assert same(got[~fin], ref[~fin])
         ok = fin & (ref.abs() + tol < 0.9 * torch.finfo(torch.float32).max) & (tol < big)
         assert ((got - ref).abs() <= tol)[ok].all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "fp16"])
+def test_wgrad_of_infinite_gradients_at_any_strides(dtype):
+    """the same where samples and rows lie at two distances; db of every row once"""
+    from yolov5m_amd.act8 import act8_load, act8_store, act8_wgrad
+    x = rows_tensor((3, 40, 21), "f32", 124)
+    dy = rows_tensor((6, 20, 21), dtype, 125)[::2]
+    dy[1, 2, 7], dy[2, 3, 20] = float("inf"), torch.finfo(DT[dtype]).max
+    kept = act8_store(x, "int8")
+    dw, db = act8_wgrad(dy, kept, bias=True)
+    xv, dv = (t.cpu().double().movedim(1, -1).flatten(0, 1) for t in (act8_load(kept), dy))
+    want, fin = dv.t() @ xv, torch.arange(20) != 2
+    assert same(dw.cpu().double()[2], want[2]) and float(db[2]) == float("inf")
+    ok = torch.isfinite(want.float())
+    assert ((dw.cpu().double() - want).abs() <= 36 * U * (dv.abs().t() @ xv.abs()))[fin][ok[fin]].all()
+    assert ((db.cpu().double() - dv.sum(0)).abs() <= 20 * U * dv.abs().sum(0))[fin].all()

@@ -175,9 +175,9 @@ template <int DT, int PA, int PC, int MODE> struct AwLoader {
 __device__ __forceinline__ unsigned aw_pair(unsigned lo, unsigned hi, int h) {
     return __builtin_amdgcn_perm(hi, lo, h ? 0x07060302u : 0x05040100u);
 }
-template <bool ON> struct AwFlag { static constexpr bool on = ON; };
-// within bf16's finite values (a NaN: any of them)
-__device__ __forceinline__ float aw_limit(float v) { return __builtin_amdgcn_fmed3f(v, -0x1.fep127f, 0x1.fep127f); }
+template <bool LIM, bool FIRST> struct AwPass { static constexpr bool lim = LIM, first = FIRST; };
+// bits of v within bf16's finite values (a NaN: any of them)
+__device__ __forceinline__ unsigned aw_limit(float v) { return __float_as_uint(__builtin_amdgcn_fmed3f(v, -0x1.fep127f, 0x1.fep127f)); }
 // two codes (bytes 2 h, 2 h + 1 of w) times their scale as a pair of bf16 (exact)
 template <int FMT> __device__ __forceinline__ unsigned aw_decode2(unsigned w, float scale, int h) {
     if constexpr (FMT == Y5M_KEEP_E4M3) {
@@ -215,9 +215,9 @@ __global__ __launch_bounds__(AW_THREADS, PA * PC <= 32 ? 2 : 1) void act8_wgrad_
     for (int k = 0; k < PA; ++k) bias[k] = 0.f;
 
     const AwLoader<DT, PA, PC, MODE> L(P, m0, m1, n0 + PA * i16, c0 + PC * i16, g, c0, i16);
-    // lim: the pieces before the last are limited to bf16's finite values
-    auto compute = [&](AwStage<DT, PA, PC>& st, auto lim) __attribute__((always_inline)) {
-        constexpr bool LIM = decltype(lim)::on;
+    // pass: are the pieces before the last limited to bf16's finite values, are these rows taken for the first time
+    auto compute = [&](AwStage<DT, PA, PC>& st, auto pass) __attribute__((always_inline)) {
+        constexpr bool LIM = decltype(pass)::lim, BIAS = DB && decltype(pass)::first;
         // (rows and channels beyond the last: codes 0, scale byte 0 = 0.0)
         aw_bf16x8 xf[PC];
         float sc[8];
@@ -247,7 +247,7 @@ __global__ __launch_bounds__(AW_THREADS, PA * PC <= 32 ? 2 : 1) void act8_wgrad_
             if constexpr (DT == Y5M_BF16) {
 #pragma unroll
                 for (int p = 0; p < 4; ++p) yf[0][p] = aw_pair(st.a[2 * p][ja >> 1], st.a[2 * p + 1][ja >> 1], ja & 1);
-                if constexpr (DB) {
+                if constexpr (BIAS) {
 #pragma unroll
                     for (int p = 0; p < 4; ++p) bias[ja] += __uint_as_float(yf[0][p] << 16) + __uint_as_float(yf[0][p] & 0xffff0000u);
                 }
@@ -263,10 +263,11 @@ __global__ __launch_bounds__(AW_THREADS, PA * PC <= 32 ? 2 : 1) void act8_wgrad_
                         lo = f16_to_f32((uint16_t)(st.a[2 * p][ja >> 1] >> (16 * (ja & 1))));
                         hi = f16_to_f32((uint16_t)(st.a[2 * p + 1][ja >> 1] >> (16 * (ja & 1))));
                     }
-                    if constexpr (DB && !LIM) bias[ja] += lo + hi;
+                    if constexpr (BIAS) bias[ja] += lo + hi;
 #pragma unroll
                     for (int e = 0; e < NP; ++e) {
-                        const unsigned w = LIM && e + 1 < NP ? f32x2_to_bf16x2(aw_limit(lo), aw_limit(hi)) : f32x2_to_bf16x2(lo, hi);
+                        // (limited pieces are truncated: rounded, the first two of the largest f32 would pass it in the sum)
+                        const unsigned w = LIM && e + 1 < NP ? aw_pair(aw_limit(lo), aw_limit(hi), 1) : f32x2_to_bf16x2(lo, hi);
                         yf[e][p] = w;
                         lo -= __uint_as_float(w << 16);
                         hi -= __uint_as_float(w & 0xffff0000u);
@@ -283,7 +284,7 @@ __global__ __launch_bounds__(AW_THREADS, PA * PC <= 32 ? 2 : 1) void act8_wgrad_
 
     // this wave's steps are rows 32 (wk + WK t) of the range; the next step's loads are in flight under the current one's products.
     // Steps are taken in pairs: one beyond the end reads zeros.
-    auto steps = [&](auto lim) __attribute__((always_inline)) {
+    auto steps = [&](auto pass) __attribute__((always_inline)) {
         const unsigned rows = (unsigned)(m1 - m0), stride = AW_K * WK;
         AwStage<DT, PA, PC> s0, s1;
         L.load(s0, AW_K * wk);
@@ -291,19 +292,21 @@ __global__ __launch_bounds__(AW_THREADS, PA * PC <= 32 ? 2 : 1) void act8_wgrad_
             // (the loads stay ahead of the products: left to itself the scheduler sinks each to its use and waits for it there)
             L.load(s1, t + stride);
             __builtin_amdgcn_sched_barrier(0);
-            compute(s0, lim);
+            compute(s0, pass);
             __builtin_amdgcn_sched_barrier(0);
             L.load(s0, t + 2 * stride);
             __builtin_amdgcn_sched_barrier(0);
-            compute(s1, lim);
+            compute(s1, pass);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    steps(AwFlag<false>());
-    if constexpr (NP > 1) {
+    constexpr bool ONCE = NP == 3 && MODE == AW_ANY && DB;
+    steps(AwPass<ONCE, true>());
+    if constexpr (NP > 1 && !ONCE) {
         // A dY that is infinite, or finite above bf16's largest value, left an infinite first piece and an opposite or NaN rest: every sum of its
         // channel is NaN. Then, and where a NaN is the right result, the wave takes its rows again with limited pieces (an infinity is left for the
-        // last one). Limiting always would cost every call 4 (fp16) to 9 % (f32).
+        // last one). Limiting always would cost every call 4 (fp16) to 9 % (f32). (ONCE: limited
+        // at once where a second loop would spill 39 registers: 255 x 100 over 1200 rows 18.1 us instead of 19.3.)
         bool nan = false;
 #pragma unroll
         for (int i = 0; i < PA; ++i)
@@ -314,7 +317,7 @@ __global__ __launch_bounds__(AW_THREADS, PA * PC <= 32 ? 2 : 1) void act8_wgrad_
             for (int i = 0; i < PA; ++i)
 #pragma unroll
                 for (int j = 0; j < PC; ++j) acc[i][j] = (aw_f32x4){0.f, 0.f, 0.f, 0.f};
-            steps(AwFlag<true>());
+            steps(AwPass<true, false>());
         }
     }
 
