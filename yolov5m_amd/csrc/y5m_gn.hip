@@ -814,7 +814,7 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_apply_kernel(const GnParams
 
 // ---- held -------------------------------------------------------------------------------------------------------------------------
 // A workgroup of up to 512 threads (256 registers each) holds a slice of `sc` channels (whole groups; whole 32-channel blocks where the 8-bit form is
-// written) of one sample: NR row pieces per thread, RP rows side by side.
+// written) of one sample: NR row pieces per thread, RP rows side by side, two plain passes over registers for mean and variance.
 // Slices of a sample follow each other on one XCD (the hardware deals workgroups round the 8 XCDs): a row's cache lines, which several
 // slices share, are fetched once.
 #define GN_HELD_THREADS 512
@@ -834,30 +834,24 @@ __device__ __forceinline__ GnSlice gn_slice(const GnParams& P) {
     w.in = w.lr < P.RP && w.nv > 0;
     return w;
 }
-// NS sums of 8 channels per thread -> tot[which][channel of the slice] in LDS. red: NS * 8 * threads values, sub: threads, tot: NS * sc
-template <int NS, typename A> __device__ __forceinline__ void gn_slice_sums(const GnParams& P, const GnSlice& w, const A* v, A* red, A* sub, A* tot) {
-    typedef A V __attribute__((ext_vector_type(16 / sizeof(A))));
-    constexpr int NV = 16 / (int)sizeof(A);
+// NS sums of 8 channels per thread -> tot[which][channel of the slice] in LDS. red: NS * 8 * threads floats, sub: threads floats,
+// tot: NS * sc floats
+template <int NS> __device__ __forceinline__ void gn_slice_sums(const GnParams& P, const GnSlice& w, const float* v, float* red, float* sub, float* tot) {
     const int T = (int)blockDim.x, wd = P.ct * 8, cols = NS * wd;
     __syncthreads();
     if (w.in) {
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-            V* d = reinterpret_cast<V*>(red + w.lr * cols + s * wd + w.lc * 8);
-#pragma unroll
-            for (int i = 0; i < 8 / NV; ++i) {
-                V t;
-#pragma unroll
-                for (int k = 0; k < NV; ++k) t[k] = v[s * 8 + i * NV + k];
-                d[i] = t;
-            }
+            float4* d = reinterpret_cast<float4*>(red + w.lr * cols + s * wd + w.lc * 8);
+            d[0] = make_float4(v[s * 8], v[s * 8 + 1], v[s * 8 + 2], v[s * 8 + 3]);
+            d[1] = make_float4(v[s * 8 + 4], v[s * 8 + 5], v[s * 8 + 6], v[s * 8 + 7]);
         }
     }
     __syncthreads();
     const int rows = P.RP < P.S ? P.RP : P.S, parts = T / cols > 0 ? T / cols : 1;
     for (int j = threadIdx.x; j < cols * parts; j += T) {
         const int part = j / cols, c = j - part * cols;
-        A a = 0;
+        float a = 0.f;
         for (int r = part; r < rows; r += parts) a += red[r * cols + c];
         if (parts > 1) sub[j] = a;
         else tot[c] = a;
@@ -865,7 +859,7 @@ template <int NS, typename A> __device__ __forceinline__ void gn_slice_sums(cons
     __syncthreads();
     if (parts > 1) {
         for (int c = threadIdx.x; c < cols; c += T) {
-            A a = 0;
+            float a = 0.f;
             for (int p = 0; p < parts; ++p) a += sub[p * cols + c];
             tot[c] = a;
         }
@@ -900,12 +894,52 @@ template <int NV, typename V, typename F> __device__ __forceinline__ void gn_sli
     }
 }
 
+// The statistics in f64, for a slice whose f32 sums may have left their range (deviations from 1e15 on, or values that are not finite
+// themselves). A thread a channel, the rows read again: rare, and small enough not to cost the usual way registers. (f64 for every slice:
+// 39 us instead of 15 for 32 x 768 x 20 x 20.) lds: 16 * ct doubles, over all that the kernel has
+template <int DT> __device__ __forceinline__ void gn_held_far(const GnParams& P, const GnSlice& w, float* lds, float* gm, float* gr) {
+    typedef typename RowElem<DT>::T T;
+    const int wd = P.ct * 8, groups = gn_div(w.nc, P.dm);
+    double* tot = reinterpret_cast<double*>(lds);
+    const int64_t ng = w.n * P.G + gn_div(w.c0, P.dm);
+    const T* x = static_cast<const T*>(P.x) + w.n * P.xn + w.c0;
+#pragma unroll 1
+    for (int c = threadIdx.x; c < w.nc; c += (int)blockDim.x) {
+        double a = 0.0, b = 0.0;
+#pragma unroll 1
+        for (int r = 0; r < P.S; ++r) {
+            const T e = x[(int64_t)r * P.xr + c];
+            double d;
+            if constexpr (DT == Y5M_F32) d = (double)e;
+            else if constexpr (DT == Y5M_BF16) d = (double)bf16_to_f32(e);
+            else d = (double)f16_to_f32(e);
+            a += d;
+            b = fma(d, d, b);
+        }
+        tot[c] = a;
+        tot[wd + c] = b;
+    }
+    __syncthreads();
+    gn_slice_groups<2>(P, w, [&](int c, int i) __attribute__((always_inline)) { return tot[i * wd + c]; }, [&](int g, const double* s) __attribute__((always_inline)) {
+        const double md = s[0] * P.inv_k, var = fma(-md, md, s[1] * P.inv_k);
+        P.mean[ng + g] = (float)md;
+        P.rstd[ng + g] = gn_rsqrt((var < 0.0 ? 0.0 : var) + (double)P.eps);          // (a NaN stays)
+    });
+    __syncthreads();                                               // (gm and gr may lie where the sums were)
+    for (int g = threadIdx.x; g < groups; g += (int)blockDim.x) {
+        gm[g] = P.mean[ng + g];
+        gr[g] = P.rstd[ng + g];
+    }
+    __syncthreads();
+}
+
 template <int DT, int AL, int FMT, int NR>
 __global__ __launch_bounds__(GN_HELD_THREADS) void gn_held_kernel(const GnParams P) {
     typedef typename RowElem<DT>::T T;
-    extern __shared__ __attribute__((aligned(16))) double lds64[];
-    double *red = lds64, *sub = red + 8 * blockDim.x, *tot = sub + blockDim.x;
-    float *gm = reinterpret_cast<float*>(tot + P.ct * 16), *gr = gm + P.ct * 8;
+    extern __shared__ __attribute__((aligned(16))) float lds[];
+    float *red = lds, *sub = red + 16 * blockDim.x, *tot = sub + blockDim.x, *gm = tot + P.ct * 16, *gr = gm + P.ct * 8;
+    __shared__ int far;                                            // did sums leave f32?
+    if (threadIdx.x == 0) far = 0;
     const GnSlice w = gn_slice(P);
     const T* b = static_cast<const T*>(P.x) + w.n * P.xn + (w.in ? w.c : w.c0);
     const int nvl = w.in ? w.nv : w.nc, lr = w.lr < P.RP ? w.lr : 0;
@@ -915,10 +949,28 @@ __global__ __launch_bounds__(GN_HELD_THREADS) void gn_held_kernel(const GnParams
         const int r = lr + i * P.RP;
         raw[i] = load_raw8<DT, AL>(b + (int64_t)(r < P.S ? r : P.S - 1) * P.xr, nvl);
     }
-    // (sums and squares in f64: gn_stats_kernel says why)
-    double a[16];
+    float a[16], m[8];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) a[k] = 0.0;
+    for (int k = 0; k < 8; ++k) a[k] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+        const bool ok = lr + i * P.RP < P.S;
+        float v[8];
+        unpack8<DT>(raw[i], v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) a[k] += ok ? v[k] : 0.f;
+    }
+    gn_slice_sums<1>(P, w, a, red, sub, tot);
+    gn_slice_groups<1>(P, w, [&](int c, int) __attribute__((always_inline)) { return (double)tot[c]; },
+                       [&](int g, const double* s) __attribute__((always_inline)) { gm[g] = (float)(s[0] * P.inv_k); });
+    __syncthreads();
+    const GnGroups gi = gn_groups(P, w.in ? w.lc * 8 : 0);         // (groups of the slice)
+    const int glast = gn_div(w.nc, P.dm) - 1;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) m[k] = gm[gi.g[k] < glast ? gi.g[k] : glast];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) a[k] = 0.f;
+    // about that mean: the squares, and the rest of the mean (what the first sum's rounding lost)
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
         const bool ok = lr + i * P.RP < P.S;
@@ -926,17 +978,17 @@ __global__ __launch_bounds__(GN_HELD_THREADS) void gn_held_kernel(const GnParams
         unpack8<DT>(raw[i], v);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const double d = (double)(ok ? v[k] : 0.f);
+            const float d = ok ? v[k] - m[k] : 0.f;
             a[k] += d;
-            a[8 + k] = fma(d, d, a[8 + k]);
+            a[8 + k] = fmaf(d, d, a[8 + k]);
         }
     }
+    gn_slice_sums<2>(P, w, a, red, sub, tot);
     const int wd = P.ct * 8;
-    gn_slice_sums<1>(P, w, a, red, sub, tot);
-    gn_slice_sums<1>(P, w, a + 8, red, sub, tot + wd);
-    gn_slice_groups<2>(P, w, [&](int c, int i) __attribute__((always_inline)) { return tot[i * wd + c]; }, [&](int g, const double* s) __attribute__((always_inline)) {
-        const double md = s[0] * P.inv_k, var = fma(-md, md, s[1] * P.inv_k);
-        const float mean = (float)md, rs = gn_rsqrt((var < 0.0 ? 0.0 : var) + (double)P.eps);          // (a NaN stays)
+    gn_slice_groups<2>(P, w, [&](int c, int i) __attribute__((always_inline)) { return (double)tot[i * wd + c]; }, [&](int g, const double* s) __attribute__((always_inline)) {
+        const double off = s[0] * P.inv_k, var = s[1] * P.inv_k - off * off;
+        const float mean = (float)((double)gm[g] + off), v = (float)((var < 0.0 ? 0.0 : var) + (double)P.eps), rs = 1.0f / sqrtf(v);          // (a NaN stays)
+        if (!(v > 1e-30f && v < 1e30f)) far = 1;
         gm[g] = mean;
         gr[g] = rs;
         const int64_t ng = w.n * P.G + gn_div(w.c0, P.dm) + g;
@@ -944,16 +996,16 @@ __global__ __launch_bounds__(GN_HELD_THREADS) void gn_held_kernel(const GnParams
         P.rstd[ng] = rs;
     });
     __syncthreads();
-    const GnGroups gi = gn_groups(P, w.in ? w.lc * 8 : 0);         // (groups of the slice)
-    const int glast = gn_div(w.nc, P.dm) - 1;
+    if (__builtin_expect(far, 0)) gn_held_far<DT>(P, w, red, gm, gr);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) m[k] = gm[gi.g[k] < glast ? gi.g[k] : glast];
     GnAffine<DT> af;
     {
         GnCoef k;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int g = gi.g[i] < glast ? gi.g[i] : glast;
-            k.mean[i] = gm[g];
-            k.rstd[i] = gr[g];
+            k.mean[i] = m[i];
+            k.rstd[i] = gr[gi.g[i] < glast ? gi.g[i] : glast];
             const int c = w.in && i < w.nv ? w.c + i : w.c0;
             k.gamma[i] = P.gamma ? P.gamma[c] : 1.0f;
             k.beta[i] = P.beta ? P.beta[c] : 0.0f;
@@ -1254,7 +1306,7 @@ template <int DT, int AL, int FMT> static int gn_fwd_split(GnParams& P, hipStrea
 template <int DT, int AL, int FMT> static int gn_fwd(GnParams& P, hipStream_t st) {
     const GnHeld h = gn_held(P, FMT != Y5M_KEEP_NONE, AL > 0, GN_FWD_ROWS, GN_HELD_FWD);
     if (h.nr == 0) return gn_fwd_split<DT, AL, FMT>(P, st);
-    const int lds = (18 * h.threads + 6 * P.ct * 8) * (int)sizeof(float);
+    const int lds = (17 * h.threads + 4 * P.ct * 8) * (int)sizeof(float);
     if (h.nr == 4) GN_HELD_LAUNCH((gn_held_kernel<DT, AL, FMT, 4>), lds);
     else GN_HELD_LAUNCH((gn_held_kernel<DT, AL, FMT, 16>), lds);
     Y5M_CHECK_LAUNCH("gn_held_kernel");
