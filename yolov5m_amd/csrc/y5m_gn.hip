@@ -938,7 +938,7 @@ __global__ __launch_bounds__(GN_HELD_THREADS) void gn_held_kernel(const GnParams
     typedef typename RowElem<DT>::T T;
     extern __shared__ __attribute__((aligned(16))) float lds[];
     float *red = lds, *sub = red + 16 * blockDim.x, *tot = sub + blockDim.x, *gm = tot + P.ct * 16, *gr = gm + P.ct * 8;
-    __shared__ int far;                                            // did sums leave f32?
+    int& far = *reinterpret_cast<int*>(gr + P.ct * 8);              // did sums leave f32?
     if (threadIdx.x == 0) far = 0;
     const GnSlice w = gn_slice(P);
     const T* b = static_cast<const T*>(P.x) + w.n * P.xn + (w.in ? w.c : w.c0);
@@ -1306,7 +1306,7 @@ template <int DT, int AL, int FMT> static int gn_fwd_split(GnParams& P, hipStrea
 template <int DT, int AL, int FMT> static int gn_fwd(GnParams& P, hipStream_t st) {
     const GnHeld h = gn_held(P, FMT != Y5M_KEEP_NONE, AL > 0, GN_FWD_ROWS, GN_HELD_FWD);
     if (h.nr == 0) return gn_fwd_split<DT, AL, FMT>(P, st);
-    const int lds = (17 * h.threads + 4 * P.ct * 8) * (int)sizeof(float);
+    const int lds = (17 * h.threads + 4 * P.ct * 8 + 4) * (int)sizeof(float);
     if (h.nr == 4) GN_HELD_LAUNCH((gn_held_kernel<DT, AL, FMT, 4>), lds);
     else GN_HELD_LAUNCH((gn_held_kernel<DT, AL, FMT, 16>), lds);
     Y5M_CHECK_LAUNCH("gn_held_kernel");
