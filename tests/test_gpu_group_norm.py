@@ -685,3 +685,22 @@ def test_statistics_over_the_whole_range_of_the_type(rows, dtype):
         z, saved = group_norm_act(x, 4, act=None, eps=eps, keep="x")
         assert ((saved.rstd.cpu().double().flatten() - ref.rstd).abs() <= 64 * U * ref.rstd).all(), (first, scale)
         near(ref, z, "z")
+
+
+@pytest.mark.parametrize("keep", ["x", "e4m3", "int8"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [3, 50, 5000])
+def test_gradients_of_very_large_inputs(rows, dtype, keep):
+    """inputs from 1e12 to 1e30, where rstd^2 and sums of dz x leave f32: the gradients are those of the normalised values, within the bounds of
+    ordinary inputs"""
+    from yolov5m_amd.group_norm import group_norm_act, group_norm_act_backward
+    for scale, offset in ((1e12, 0.0), (1e25, 0.0), (1e30, 0.0), (1e20, 1e21)):
+        x = (torch.randn((2, rows, 16), generator=torch.Generator().manual_seed(112)) * scale + offset).to(DT[dtype]).movedim(-1, 1).to(DEV)
+        dz = (_rows((2, 16, rows), "f32", 113) * 1e10).to(DT[dtype])
+        ga, be = _params(16, 114)
+        kept = None if keep == "x" else stored_values(x, keep)[0]
+        ref = Exact(x, 4, ga, be, 1e-3, "silu", kept, dz)
+        z, saved = group_norm_act(x, 4, ga, be, eps=1e-3, keep=keep)
+        near(ref, z, "z")
+        for got, what in zip(group_norm_act_backward(dz, saved), ("dx", "dgamma", "dbeta")):
+            near(ref, got, what)
