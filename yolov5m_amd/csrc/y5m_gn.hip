@@ -539,14 +539,14 @@ template <int DT> __device__ __forceinline__ void gn_coef_xhat(GnCoef& k) {
     }
 }
 
-// dt = dz act'(t) of one piece. XH: through xhat, which comes back in v (f32; bf16 where gn_far). Else v stays the kept value and
-// u = -t log2(e) is one fma of it (GnAffine says why that is enough): act'(t) = s (1 + t (1 - s)), s = 1 / (1 + 2^u), t (1 - s) = u (ln2 s - ln2)
-template <int DT, bool XH> struct GnGrad {
-    float a[8], b[8], m[XH ? 8 : 1], r[XH ? 8 : 1];
+// dt = dz act'(t) of one piece. f32: through xhat, which comes back in v. 16 bits: v stays the kept value and u = -t log2(e) is one
+// fma of it (GnAffine says why that is enough): act'(t) = s (1 + t (1 - s)), s = 1 / (1 + 2^u), t (1 - s) = u (ln2 s - ln2)
+template <int DT> struct GnGrad {
+    float a[8], b[8], m[DT == Y5M_F32 ? 8 : 1], r[DT == Y5M_F32 ? 8 : 1];
     __device__ __forceinline__ void set(const GnCoef& k) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            if constexpr (XH) {
+            if constexpr (DT == Y5M_F32) {
                 a[i] = k.gamma[i];
                 b[i] = k.beta[i];
                 m[i] = k.mean[i];
@@ -561,7 +561,7 @@ template <int DT, bool XH> struct GnGrad {
     template <bool SILU> __device__ __forceinline__ void operator()(float* v, float* g) const {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            if constexpr (XH) {
+            if constexpr (DT == Y5M_F32) {
                 v[i] = (v[i] - m[i]) * r[i];
                 if constexpr (SILU) g[i] *= gn_act_grad<DT>(true, fmaf(v[i], a[i], b[i]));
             } else if constexpr (SILU) {
@@ -573,14 +573,10 @@ template <int DT, bool XH> struct GnGrad {
         }
     }
 };
-// bf16 reaches as far as f32: where a group's values do, sums of dt x and products with rstd^2 would leave f32's range. Such rows go through
-// xhat, one at a time: within the registers of the usual way, which all channels below 2^40 take. (xhat for all of bf16: 16 registers more, and
-// with the waves they cost 526 us instead of 450 for a step over 64 x 160 x 160 x 96 in int8.)
-// waves per SIMD of the backward's passes in bf16: what the usual way needs by itself (the far one spills instead: step over
-// 64 x 40 x 40 x 384 in e4m3 136.4 us, 143 at a wave less)
-template <int DT, int AL, int FMT> constexpr int gn_bwd_waves(int aligned) {
-    return DT != Y5M_BF16 ? 1 : AL > 0 ? aligned : AL == 0 ? 4 : FMT != Y5M_KEEP_NONE ? 3 : 2;
-}
+
+// bf16 reaches as far as f32: where a group's values do, sums of dt x (they come out infinite or NaN) and products with rstd^2 (gn_far) leave
+// f32's range. Such channels are taken one by one through xhat: rare, and small enough to leave the usual way its registers. (xhat for all
+// of bf16: 16 registers more, and with the waves they cost 526 us instead of 450 for a step over 64 x 160 x 160 x 96 in int8.)
 template <int DT> __device__ __forceinline__ bool gn_far(const GnCoef& k) {
     bool far = false;
     if constexpr (DT == Y5M_BF16) {
@@ -589,11 +585,31 @@ template <int DT> __device__ __forceinline__ bool gn_far(const GnCoef& k) {
     }
     return far;
 }
+// f(row, dt, xhat) of channel c over the thread's rows
+template <int FMT, typename F> __device__ __forceinline__ void gn_far_rows(const GnParams& P, const GnPlace& w, int c, F f) {
+    const int64_t ng = w.n * P.G + gn_div(c, P.dm);
+    const float mean = P.mean[ng], rstd = P.rstd[ng], gamma = P.gamma ? P.gamma[c] : 1.0f, beta = P.beta ? P.beta[c] : 0.0f;
+#pragma unroll 1
+    for (int r = w.r0 + w.lr; r < w.r1; r += P.RP) {
+        const int64_t row = w.n * P.S + r;
+        float v;
+        if constexpr (FMT == Y5M_KEEP_NONE) {
+            v = bf16_to_f32(static_cast<const bf16_t*>(P.x)[w.n * P.xn + (int64_t)r * P.xr + c]);
+        } else {
+            const uint8_t q = P.q[row * P.ldq + c];
+            const float scale = act8_scale(P.scale[row * P.CB + (c >> 5)]);
+            if constexpr (FMT == Y5M_KEEP_E4M3) v = __builtin_amdgcn_cvt_pk_f32_fp8((int)q, false)[0] * scale;
+            else v = (float)(int8_t)q * scale;
+        }
+        const float xh = (v - mean) * rstd, dz = bf16_to_f32(static_cast<const bf16_t*>(P.dz)[w.n * P.zn + (int64_t)r * P.zr + c]);
+        f(r, dz * gn_act_grad<Y5M_BF16>(P.act == Y5M_ACT_SILU, fmaf(xh, gamma, beta)), xh);
+    }
+}
 
-template <int DT, int AL, int FMT, bool SILU, bool XH>
+template <int DT, int AL, int FMT, bool SILU>
 __device__ __forceinline__ void gn_bwd_sums(const GnParams& P, const GnPlace& w, const GnGroups& gr, float* a) {
     typedef typename RowElem<DT>::T T;
-    GnGrad<DT, XH> grad;
+    GnGrad<DT> grad;
     {
         GnCoef k;
         gn_coef(P, w, gr, k);
@@ -613,50 +629,68 @@ __device__ __forceinline__ void gn_bwd_sums(const GnParams& P, const GnPlace& w,
     int r = w.r0 + w.lr;
     GnCursor<DT, AL, FMT> at(P, w, r, static_cast<const T*>(P.dz) + w.n * P.zn + w.c);
     // (two rows in flight: four cost a quarter of the waves and 30 % of the time)
-    if constexpr (DT == Y5M_F32 || !XH)
-        for (; r + P.RP < w.r1; r += 2 * P.RP) {
-            GnKept<DT, FMT> kept[2];
-            Raw8<DT> graw[2];
+    for (; r + P.RP < w.r1; r += 2 * P.RP) {
+        GnKept<DT, FMT> kept[2];
+        Raw8<DT> graw[2];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) at.next(kept[u], graw[u]);
+        for (int u = 0; u < 2; ++u) at.next(kept[u], graw[u]);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) add(kept[u], graw[u]);
-        }
+        for (int u = 0; u < 2; ++u) add(kept[u], graw[u]);
+    }
     for (; r < w.r1; r += P.RP) {
         GnKept<DT, FMT> kept;
         Raw8<DT> graw;
         at.next(kept, graw);
         add(kept, graw);
     }
-    if constexpr (!XH) {
-        // sum dt x -> sum dt xhat. (Are the values far? Asked here, where the statistics are at hand, it keeps the loads of the first rows early)
+    if constexpr (DT != Y5M_F32) {
+        // sum dt x -> sum dt xhat
         GnCoef k;
         gn_stat8(P, w, gr, k);
-        if (gn_far<DT>(k)) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) a[i] = 0.f;
-            gn_bwd_sums<DT, AL, FMT, SILU, true>(P, w, gr, a);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) a[8 + i] = k.rstd[i] * fmaf(-k.mean[i], a[i], a[8 + i]);
-        }
+        for (int i = 0; i < 8; ++i) a[8 + i] = k.rstd[i] * fmaf(-k.mean[i], a[i], a[8 + i]);
     }
 }
 
 template <int DT, int AL, int FMT>
-__global__ __launch_bounds__(GN_THREADS, (gn_bwd_waves<DT, AL, FMT>(4))) void gn_bwd_reduce_kernel(const GnParams P) {
+__global__ __launch_bounds__(GN_THREADS) void gn_bwd_reduce_kernel(const GnParams P) {
     __shared__ __attribute__((aligned(16))) float red[GN_THREADS * 16];
+    __shared__ int far;
     const GnPlace w = gn_place<false>(P, P.rpc);
     if (w.n >= P.N) return;
+    if (DT == Y5M_BF16 && threadIdx.x == 0) far = 0;
     float a[16];
 #pragma unroll
     for (int k = 0; k < 16; ++k) a[k] = 0.f;
     if (w.in) {
         const GnGroups gr = gn_groups(P, w.c);
-        if (P.act == Y5M_ACT_SILU) gn_bwd_sums<DT, AL, FMT, true, DT == Y5M_F32>(P, w, gr, a);
-        else gn_bwd_sums<DT, AL, FMT, false, DT == Y5M_F32>(P, w, gr, a);
+        if (P.act == Y5M_ACT_SILU) gn_bwd_sums<DT, AL, FMT, true>(P, w, gr, a);
+        else gn_bwd_sums<DT, AL, FMT, false>(P, w, gr, a);
     }
-    gn_join_rows(a, red, w, P.ct, P.RP, P.C, [&](int c, float s0, float s1) __attribute__((always_inline)) { *gn_part(P, w, c) = make_float2(s0, s1); });
+    gn_join_rows(a, red, w, P.ct, P.RP, P.C, [&](int c, float s0, float s1) __attribute__((always_inline)) {
+        *gn_part(P, w, c) = make_float2(s0, s1);
+        if (DT == Y5M_BF16 && !(fabsf(s1) < INFINITY)) far = 1;
+    });
+    if constexpr (DT == Y5M_BF16) {
+        // (asked last, where nothing of the loop is held any more: asked before it, or between it and the join, it cost 4 to 10 %)
+        __syncthreads();
+        if (__builtin_expect(far, 0)) {
+            for (int i = 0; i < 8; ++i) {
+                float s0 = 0.f, s1 = 0.f;
+                if (w.in && i < w.nv)
+                    gn_far_rows<FMT>(P, w, w.c + i, [&](int, float dt, float xh) __attribute__((always_inline)) {
+                        s0 += dt;
+                        s1 = fmaf(dt, xh, s1);
+                    });
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    a[j] = i == j ? s0 : a[j];
+                    a[8 + j] = i == j ? s1 : a[8 + j];
+                }
+            }
+            gn_join_rows(a, red, w, P.ct, P.RP, P.C, [&](int c, float s0, float s1) __attribute__((always_inline)) { *gn_part(P, w, c) = make_float2(s0, s1); });
+        }
+    }
 }
 
 // channel sums of a sample and A, B of its groups, one workgroup per (sample, group)
@@ -743,21 +777,41 @@ __global__ __launch_bounds__(GN_THREADS) void gn_param_grad_kernel(const GnParam
     }
 }
 
-template <int DT, int AL, int FMT, bool SILU, bool XH>
-__device__ __forceinline__ void gn_bwd_rows(const GnParams& P, const GnPlace& w, const GnCoef& k, const float2* ab) {
+template <int DT, int AL, int FMT, bool SILU, bool INL>
+__device__ __forceinline__ void gn_bwd_rows(const GnParams& P, const GnPlace& w, const float2* lab, int g0) {
     typedef typename RowElem<DT>::T T;
-    // dx = r gamma dt - r A - r B xhat = c1 dt + (c2 v + c3), v = xhat (XH) or the kept value
-    GnGrad<DT, XH> grad;
-    grad.set(k);
+    // dx = r gamma dt - r A - r B xhat = c1 dt + (c2 v + c3), v = xhat in f32, the kept value in 16 bits
+    GnGrad<DT> grad;
     float c1[8], c2[8], c3[8];
+    {
+        const GnGroups gr = gn_groups(P, w.c);
+        GnCoef k;
+        gn_coef(P, w, gr, k);
+        if (__builtin_expect(gn_far<DT>(k), 0)) {
+            const float2* ab = INL ? lab - g0 : reinterpret_cast<const float2*>(P.ab) + w.n * P.G;
+#pragma unroll 1
+            for (int i = 0; i < 8 && i < w.nv; ++i) {
+                const int c = w.c + i, g = gn_div(c, P.dm);
+                const float r = P.rstd[w.n * P.G + g], A = ab[g].x, B = ab[g].y, ga = P.gamma ? P.gamma[c] : 1.0f;
+                gn_far_rows<FMT>(P, w, c, [&](int row, float dt, float xh) __attribute__((always_inline)) {
+                    static_cast<bf16_t*>(P.out)[w.n * P.on + (int64_t)row * P.orow + c] = f32_to_bf16(r * (ga * dt - A - xh * B));
+                });
+            }
+            return;
+        }
+        grad.set(k);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        c1[i] = k.rstd[i] * k.gamma[i];
-        c2[i] = -k.rstd[i] * ab[i].y;
-        c3[i] = -k.rstd[i] * ab[i].x;
-        if constexpr (!XH) {
-            c2[i] *= k.rstd[i];
-            c3[i] = fmaf(-c2[i], k.mean[i], c3[i]);
+        for (int i = 0; i < 8; ++i) {
+            // (channels behind the last: any of the tile's groups)
+            const int g = gr.g[i];
+            const float2 ab = INL ? lab[g - g0] : *reinterpret_cast<const float2*>(P.ab + (w.n * P.G + g) * 2);
+            c1[i] = k.rstd[i] * k.gamma[i];
+            c2[i] = -k.rstd[i] * ab.y;
+            c3[i] = -k.rstd[i] * ab.x;
+            if constexpr (DT != Y5M_F32) {
+                c2[i] *= k.rstd[i];
+                c3[i] = fmaf(-c2[i], k.mean[i], c3[i]);
+            }
         }
     }
     auto finish = [&](const GnKept<DT, FMT>& kept, const Raw8<DT>& graw, T* to) __attribute__((always_inline)) {
@@ -773,29 +827,27 @@ __device__ __forceinline__ void gn_bwd_rows(const GnParams& P, const GnPlace& w,
     GnCursor<DT, AL, FMT> at(P, w, r, static_cast<const T*>(P.dz) + w.n * P.zn + w.c);
     T* op = static_cast<T*>(P.out) + w.n * P.on + (int64_t)r * P.orow + w.c;
     const int64_t ostep = (int64_t)P.RP * P.orow;
-    if constexpr (DT == Y5M_F32 || !XH)
-        for (; r + P.RP < w.r1; r += 2 * P.RP) {
-            GnKept<DT, FMT> kept[2];
-            Raw8<DT> graw[2];
+    for (; r + P.RP < w.r1; r += 2 * P.RP) {
+        GnKept<DT, FMT> kept[2];
+        Raw8<DT> graw[2];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) at.next(kept[u], graw[u]);
+        for (int u = 0; u < 2; ++u) at.next(kept[u], graw[u]);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                finish(kept[u], graw[u], op);
-                op += ostep;
-            }
+        for (int u = 0; u < 2; ++u) {
+            finish(kept[u], graw[u], op);
+            op += ostep;
         }
-    for (; r < w.r1; r += P.RP) {
+    }
+    if (r < w.r1) {
         GnKept<DT, FMT> kept;
         Raw8<DT> graw;
         at.next(kept, graw);
         finish(kept, graw, op);
-        op += ostep;
     }
 }
 
 template <int DT, int AL, int FMT, bool INL>
-__global__ __launch_bounds__(GN_THREADS, (gn_bwd_waves<DT, AL, FMT>(FMT != Y5M_KEEP_NONE ? 5 : 4))) void gn_bwd_apply_kernel(const GnParams P) {
+__global__ __launch_bounds__(GN_THREADS) void gn_bwd_apply_kernel(const GnParams P) {
     const GnPlace w = gn_place<true>(P, P.arpc);
     if (w.n < 0) return;
     const float2* lab = nullptr;
@@ -825,24 +877,8 @@ __global__ __launch_bounds__(GN_THREADS, (gn_bwd_waves<DT, AL, FMT>(FMT != Y5M_K
         __syncthreads();
     }
     if (!w.in) return;
-    const GnGroups gr = gn_groups(P, w.c);
-    GnCoef k;
-    gn_coef(P, w, gr, k);
-    float2 c[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        // (channels behind the last: any of the tile's groups)
-        const int g = gr.g[i];
-        c[i] = INL ? lab[g - g0] : *reinterpret_cast<const float2*>(P.ab + (w.n * P.G + g) * 2);
-    }
-    const bool silu = P.act == Y5M_ACT_SILU;
-    if (DT == Y5M_F32 || gn_far<DT>(k)) {
-        if (silu) gn_bwd_rows<DT, AL, FMT, true, true>(P, w, k, c);
-        else gn_bwd_rows<DT, AL, FMT, false, true>(P, w, k, c);
-    } else if constexpr (DT != Y5M_F32) {
-        if (silu) gn_bwd_rows<DT, AL, FMT, true, false>(P, w, k, c);
-        else gn_bwd_rows<DT, AL, FMT, false, false>(P, w, k, c);
-    }
+    if (P.act == Y5M_ACT_SILU) gn_bwd_rows<DT, AL, FMT, true, INL>(P, w, lab, g0);
+    else gn_bwd_rows<DT, AL, FMT, false, INL>(P, w, lab, g0);
 }
 
 // ---- held -------------------------------------------------------------------------------------------------------------------------
