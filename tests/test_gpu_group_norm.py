@@ -704,3 +704,26 @@ def test_gradients_of_very_large_inputs(rows, dtype, keep):
         near(ref, z, "z")
         for got, what in zip(group_norm_act_backward(dz, saved), ("dx", "dgamma", "dbeta")):
             near(ref, got, what)
+
+
+@pytest.mark.parametrize("keep", ["e4m3", "int8"])
+def test_cbl_keeps_nothing_where_no_gradient_is_wanted(keep, monkeypatch):
+    """no_grad, inference_mode and a frozen weight store no input in 8 bits; results are those of a training forward, up to the order in which the
+    statistics are summed (a slice is cut at whole blocks only where codes are written): each is within 64 u of |xhat| + |mean| rstd <= 6 + 1
+    of the formula, so the two within 128 u 7 = 5.4e-5"""
+    from yolov5m_amd import act8
+    from yolov5m_amd.model import CBL
+    real, calls = act8.act8_store, []
+    monkeypatch.setattr(act8, "act8_store", lambda *a, **k: (calls.append(1), real(*a, **k))[1])
+    m = CBL(16, 24, 3, 1, 1, norm_groups=8, keep=keep).to(DEV)
+    x = torch.randn(2, 16, 6, 5, generator=torch.Generator().manual_seed(118)).to(DEV)
+    want = m(x)
+    assert len(calls) == 1
+    m.eval()
+    for mode in (torch.no_grad, torch.inference_mode):
+        with mode():
+            assert (m(x) - want).abs().max() <= 5.4e-5
+    assert len(calls) == 1
+    m.cbl[0].weight.requires_grad_(False)
+    m(x).sum().backward()                                             # (the norm's parameters still train)
+    assert len(calls) == 1 and m.cbl[1].weight.grad is not None

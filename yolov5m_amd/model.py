@@ -51,7 +51,8 @@ class CBL(nn.Module):
         _lib.require_cuda(x)
         conv, bn = self.cbl[0], self.cbl[1]
         if self.norm_groups is not None:
-            return bn(_ConvKeptFn.apply(x.float(), conv.weight, self)).float()
+            keep_input = torch.is_grad_enabled() and conv.weight.requires_grad          # (inside the function grad mode is always off)
+            return bn(_ConvKeptFn.apply(x.float(), conv.weight, self, keep_input)).float()
         return _CBLFn.apply(x.float(), conv.weight, bn.weight, bn.bias, self)
 
 
@@ -61,7 +62,7 @@ class _ConvKeptFn(torch.autograd.Function):
     from the values read back (act8_load)"""
 
     @staticmethod
-    def forward(ctx, x, w, mod):
+    def forward(ctx, x, w, mod, keep_input=True):
         from . import ops
         from .act8 import act8_store
         conv, keep, dtype = mod.cbl[0], mod.cbl[1].keep, mod.compute_dtype
@@ -78,7 +79,7 @@ class _ConvKeptFn(torch.autograd.Function):
         ctx.geom = (k, s, p, dtype, cin, tuple(x.shape[2:]))
         ctx.act8 = None
         kept = [None, None]
-        if ctx.needs_input_grad[1]:                           # (the input is read by the weight gradient only)
+        if keep_input and ctx.needs_input_grad[1]:            # (the input is read by the weight gradient only)
             if keep == "x":
                 kept = [xd, None]
             else:
@@ -107,7 +108,7 @@ class _ConvKeptFn(torch.autograd.Function):
             else:
                 dw = ops.conv_wgrad(dy.float(), act8_load(Act8(xk, scale, *ctx.act8)).float(), k, s, p, dtype)
             dw = dw[:, :cin]
-        return dx, dw, None
+        return dx, dw, None, None
 
 
 class _CBLFn(torch.autograd.Function):
