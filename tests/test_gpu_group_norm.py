@@ -727,3 +727,16 @@ def test_cbl_keeps_nothing_where_no_gradient_is_wanted(keep, monkeypatch):
     m.cbl[0].weight.requires_grad_(False)
     m(x).sum().backward()                                             # (the norm's parameters still train)
     assert len(calls) == 1 and m.cbl[1].weight.grad is not None
+
+
+@pytest.mark.parametrize("frozen", [True, False])
+def test_forward_mode_is_refused(frozen):
+    """a tangent is never dropped silently: with frozen parameters (no autograd node) and with trained ones"""
+    import torch.autograd.forward_ad as fw
+    from yolov5m_amd.group_norm import GroupNormAct
+    layer = GroupNormAct(4, 16).to(DEV).requires_grad_(not frozen)
+    x = _rows((2, 16, 3, 3), "f32", 119)
+    with fw.dual_level():
+        with pytest.raises((RuntimeError, NotImplementedError), match="forward|jvp"):
+            layer(fw.make_dual(x, torch.ones_like(x)))
+        assert fw.unpack_dual(layer(x)).tangent is None

@@ -12,6 +12,7 @@ fixed order. Types: float32, bfloat16, float16 for x / z / dz / dx; weight and b
 """
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import Y5MError, c_float, c_int, c_int64, c_size_t, c_void_p, register
@@ -60,7 +61,9 @@ def _ptr(t):
 
 def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="silu", keep=None):
     """z = act(weight * (x - mean) / sqrt(var + eps) + bias), mean and (biased) variance per sample and group of C / groups
-    consecutive channels. Returns (z, saved); saved is None without `keep`."""
+    consecutive channels. Returns (z, saved); saved is None without `keep`. Autograd does not record the call: z carries no gradient,
+    group_norm_act_backward(dz, saved) gives them (weight and bias are read again there: change them only behind it). GroupNormAct is
+    the form that autograd records."""
     _lib.require_cuda(x)
     n, s, c, sn, sr = rows_of(x, "x")
     if not isinstance(groups, int) or groups < 1 or c % groups:
@@ -178,6 +181,8 @@ class GroupNormAct(nn.Module):
     def forward(self, x):
         needs = torch.is_grad_enabled() and (x.requires_grad or (self.weight is not None and (self.weight.requires_grad or self.bias.requires_grad)))
         if not needs:
+            if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (x, self.weight, self.bias)):
+                raise Y5MError("GroupNormAct has no forward-mode derivative: its output would carry no tangent")
             return group_norm_act(x, self.groups, self.weight, self.bias, self.eps, self.act)[0]
         return _GroupNormActFn.apply(x, self.weight, self.bias, self.groups, self.eps, self.act, self.keep)
 
