@@ -462,6 +462,7 @@ int y5m_act8_wgrad(const void* dy, int64_t dy_batch_stride, int64_t dy_row_strid
  * N samples of S rows of C channels in G groups; strides in elements, channels dense, any strides for inputs (views of wider
  * buffers); gamma / beta may be NULL (1, 0). mean / rstd [N][G] f32 are outputs of the forward and inputs of the backward.
  * fmt != Y5M_KEEP_NONE: the forward also writes the 8-bit form of x (q, scale; row = n * S + s) and the backward reads it instead of x.
+ * Workspaces: 0 bytes where one launch holds the map (ws may be NULL then), else 16-byte aligned, one per call in flight.
  * z may be x itself, dx may be x or dz (equal strides). The backward OVERWRITES dgamma / dbeta (NULL: not wanted); no atomics, one result per input. */
 size_t y5m_gn_act_workspace_bytes(int64_t N, int64_t S, int C, int G);
 int y5m_gn_act(const void* x, int64_t x_batch_stride, int64_t x_row_stride, const float* gamma, const float* beta, int64_t N, int64_t S,

@@ -740,3 +740,51 @@ def test_forward_mode_is_refused(frozen):
         with pytest.raises((RuntimeError, NotImplementedError), match="forward|jvp"):
             layer(fw.make_dual(x, torch.ones_like(x)))
         assert fw.unpack_dual(layer(x)).tangent is None
+
+
+@pytest.mark.parametrize("case", [((16384, 768), 32, True), ((3, 64, 5, 5), 4, True), ((1, 768, 20, 20), 32, False), ((2, 24, 37), 3, True), ((2, 96, 130, 50), 32, False),
+                                  ((1, 8, 5000), 1, False)])
+def test_workspace_of_the_form_that_runs(case):
+    """maps that one launch holds need no workspace forward, and none is touched; a null pointer is taken there. Longer ones, and the backward,
+    write within what the size functions say, whatever the alignment and the kept form. (One 20 x 20 x 768 map is held without an 8-bit form
+    only: with one its slices are whole blocks, lcm(24, 32) = 96 channels wide, and eight workgroups are too few for 16 rows a thread.)"""
+    import yolov5m_amd.group_norm  # noqa: F401
+    from yolov5m_amd import _lib
+    from yolov5m_amd.act8 import FORMATS
+    L = _lib.lib()
+    (n, c, *sp), g, held = case
+    s = 1
+    for v in sp:
+        s *= v
+    wsb, bwb = L.y5m_gn_act_workspace_bytes(n, s, c, g), L.y5m_gn_act_bwd_workspace_bytes(n, s, c, g)
+    assert (wsb == 0) == held and bwb >= 8 * n * c
+    if held:
+        assert bwb <= 8 * n * (c + g)
+    if DEV != "cuda" and n * c * s > 10 ** 6:
+        return
+    ldq, cb = -(-c // 8) * 8, -(-c // 32)
+    for odd in (0, 1):
+        buf = torch.randn(n * s * c + odd, generator=torch.Generator().manual_seed(128)).to(DEV)
+        x = buf[odd:].view(n, s, c)
+        ref = Exact(x.transpose(1, 2), g, None, None, 1e-5, "silu", None, x.transpose(1, 2))
+        for fmt in (0, *FORMATS.values()):
+            z, dx = torch.empty((n, s, c), device=DEV), torch.empty((n, s, c), device=DEV)
+            stat = torch.empty(2 * n * g, device=DEV)
+            q, sc = torch.empty((n * s, ldq), dtype=torch.uint8, device=DEV), torch.empty((n * s, cb), dtype=torch.uint8, device=DEV)
+            ws, bw = (torch.full((b + 64,), 7, dtype=torch.uint8, device=DEV) for b in (wsb, bwb))
+            p = stat.data_ptr()
+            _lib.check(L.y5m_gn_act(x.data_ptr(), s * c, c, None, None, n, s, c, g, 1e-5, 1, z.data_ptr(), s * c, c, p, p + 4 * n * g, q.data_ptr() if fmt else None,
+                                    ldq, sc.data_ptr() if fmt else None, fmt, None if held else ws.data_ptr(), wsb, 0, _lib.stream_ptr()), "y5m_gn_act")
+            near(ref, z.transpose(1, 2), "z")
+            _lib.check(L.y5m_gn_act_bwd(x.data_ptr(), s * c, c, x.data_ptr(), s * c, c, q.data_ptr() if fmt else None, ldq, sc.data_ptr() if fmt else None, fmt, None,
+                                        None, p, p + 4 * n * g, n, s, c, g, 1, dx.data_ptr(), s * c, c, None, None, bw.data_ptr(), bwb, 0, _lib.stream_ptr()),
+                       "y5m_gn_act_bwd")
+            if fmt == 0:
+                near(ref, dx.transpose(1, 2), "dx")
+            assert (ws[wsb:] == 7).all() and (bw[bwb:] == 7).all()
+    # one byte too few is refused
+    if not held:
+        assert L.y5m_gn_act(x.data_ptr(), s * c, c, None, None, n, s, c, g, 1e-5, 1, z.data_ptr(), s * c, c, p, p + 4 * n * g, None, 0, None, 0, ws.data_ptr(), wsb - 1, 0,
+                            _lib.stream_ptr()) != 0
+    assert L.y5m_gn_act_bwd(x.data_ptr(), s * c, c, x.data_ptr(), s * c, c, None, 0, None, 0, None, None, p, p + 4 * n * g, n, s, c, g, 1, dx.data_ptr(), s * c, c, None,
+                            None, bw.data_ptr(), bwb - 1, 0, _lib.stream_ptr()) != 0

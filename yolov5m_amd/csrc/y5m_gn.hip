@@ -1306,14 +1306,27 @@ static void gn_sizes(GnParams& P, int64_t N, int64_t S, int C, int G) {
     P.inv_k = 1.0 / ((double)S * (double)P.D);
 }
 
-extern "C" size_t y5m_gn_act_workspace_bytes(int64_t N, int64_t S, int C, int G) {
-    if (N <= 0 || S <= 0 || C <= 0 || G <= 0 || C % G || S >= (1ll << 30) || N >= (1ll << 30)) return 0;
-    GnParams P = {};
-    gn_sizes(P, N, S, C, G);
+static bool gn_no_sizes(int64_t N, int64_t S, int C, int G) {
+    return N <= 0 || S <= 0 || C <= 0 || C >= (1 << 16) || G <= 0 || C % G || S >= (1ll << 30) || N >= (1ll << 30);
+}
+// the split form's sums, for the alignment and 8-bit form that need most
+static size_t gn_part_bytes(GnParams P) {
     gn_geometry(P, true, GN_ROWS, GN_APPLY_ROWS);
     const int64_t a = P.chunks;
     gn_geometry(P, false, GN_ROWS, GN_APPLY_ROWS);
-    return (size_t)N * (size_t)(a > P.chunks ? a : P.chunks) * 2 * C * sizeof(float);
+    return (size_t)P.N * (size_t)(a > P.chunks ? a : P.chunks) * 2 * P.C * sizeof(float);
+}
+// does the held form run whatever the alignment and the 8-bit form are?
+static bool gn_always_held(GnParams P, bool forward) {
+    const int* nrs = forward ? GN_FWD_ROWS : GN_BWD_ROWS;
+    const int64_t most = forward ? GN_HELD_FWD : GN_HELD_BWD;
+    return gn_held(P, false, false, nrs, most).nr && gn_held(P, false, true, nrs, most).nr && (!forward || gn_held(P, true, true, nrs, most).nr);
+}
+extern "C" size_t y5m_gn_act_workspace_bytes(int64_t N, int64_t S, int C, int G) {
+    if (gn_no_sizes(N, S, C, G)) return 0;
+    GnParams P = {};
+    gn_sizes(P, N, S, C, G);
+    return gn_always_held(P, true) ? 0 : gn_part_bytes(P);
 }
 
 #define GN_DT(GO)                                                                    \
@@ -1396,7 +1409,8 @@ extern "C" int y5m_gn_act(const void* x, int64_t x_batch_stride, int64_t x_row_s
     Y5M_REQUIRE(z != x || (z_batch_stride == x_batch_stride && z_row_stride == x_row_stride), "in place needs equal strides");
     Y5M_REQUIRE((S == 1 || z_row_stride >= C) && (N == 1 || z_batch_stride >= (S - 1) * z_row_stride + C), "rows of the output overlap");
     if (fmt != Y5M_KEEP_NONE) Y5M_REQUIRE(q && scale && ldq >= C && ldq % 8 == 0 && ((uintptr_t)q & 7) == 0, "8-bit form: ldq % 8 == 0, at least C, codes 8-byte aligned");
-    Y5M_REQUIRE(ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= y5m_gn_act_workspace_bytes(N, S, C, G), "workspace too small or not 16-byte aligned");
+    const size_t need = y5m_gn_act_workspace_bytes(N, S, C, G);
+    Y5M_REQUIRE(need == 0 || (ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= need), "workspace too small or not 16-byte aligned");
     GnParams P = {};
     gn_sizes(P, N, S, C, G);
     P.x = x; P.out = z; P.gamma = gamma; P.beta = beta; P.mean = mean; P.rstd = rstd; P.eps = eps; P.act = act;
@@ -1412,8 +1426,11 @@ extern "C" int y5m_gn_act(const void* x, int64_t x_batch_stride, int64_t x_row_s
 }
 
 extern "C" size_t y5m_gn_act_bwd_workspace_bytes(int64_t N, int64_t S, int C, int G) {
-    if (N <= 0 || S <= 0 || C <= 0 || G <= 0 || C % G || S >= (1ll << 30) || N >= (1ll << 30)) return 0;
-    return y5m_gn_act_workspace_bytes(N, S, C, G) + ((size_t)N * 2 * C + (size_t)N * G * 2) * sizeof(float);
+    if (gn_no_sizes(N, S, C, G)) return 0;
+    GnParams P = {};
+    gn_sizes(P, N, S, C, G);
+    const size_t nc = (size_t)N * 2 * C * sizeof(float);
+    return gn_always_held(P, false) ? nc : nc + (size_t)N * G * 2 * sizeof(float) + gn_part_bytes(P);
 }
 
 template <int DT, int AL, int FMT> static int gn_bwd(GnParams& P, hipStream_t st) {
