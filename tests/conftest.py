@@ -46,11 +46,21 @@ _NOT_YET_ON_HARDWARE = {
 }
 
 
+def _full_size_gradients(module):
+    def check():
+        _, checked_dx, _, kinds = module._per_layer_backward(64, 640, one_per_shape=True)
+        assert checked_dx >= 8 and "bwd_pw" not in kinds
+    return check
+
+
 def pytest_collection_modifyitems(config, items):
     # test_bf16_train_step_backward_variants_subprocess runs this suite's "per_layer_backward" tests in a child with the fused pointwise
-    # backward switched off (Y5M_BWD_PW=0). The full-size one asserts that the DEFAULT dispatch runs that kernel, so it is no test there.
+    # backward switched off (Y5M_BWD_PW=0). Of the full-size one the gradients are checked there; which kernels the DEFAULT dispatch
+    # takes is not its question.
     if os.environ.get("Y5M_VARIANT_CHILD") == "1" and os.environ.get("Y5M_BWD_PW") == "0":
-        items[:] = [it for it in items if getattr(it, "originalname", it.name) != "test_bf16_per_layer_backward_full_size_default_dispatch"]
+        for it in items:
+            if getattr(it, "originalname", it.name) == "test_bf16_per_layer_backward_full_size_default_dispatch":
+                it.obj = _full_size_gradients(it.module)
 
     def rank(it):
         if "test_gpu_zz_dp" in it.nodeid:
