@@ -788,3 +788,44 @@ def test_workspace_of_the_form_that_runs(case):
                             _lib.stream_ptr()) != 0
     assert L.y5m_gn_act_bwd(x.data_ptr(), s * c, c, x.data_ptr(), s * c, c, None, 0, None, 0, None, None, p, p + 4 * n * g, n, s, c, g, 1, dx.data_ptr(), s * c, c, None,
                             None, bw.data_ptr(), bwb - 1, 0, _lib.stream_ptr()) != 0
+
+
+@pytest.mark.parametrize("keep", ["x", "e4m3", "int8"])
+@pytest.mark.parametrize("case", [(16, 32, 1, 1), (16, 24, 3, 1), (16, 32, 3, 2), (3, 16, 3, 1)])
+def test_cbl_with_group_norm_in_bf16(case, keep):
+    """the block's bf16 path, stage by stage against 64 bits on the operands that the stage before left: convolution output (bf16: half a step,
+    2^-8, of sums of at most 288 products in f32, 300 u), norm and its gradient (Exact's bounds), and the convolution's gradients, whose bounds
+    carry the error of the bf16 dy on: sum |err dy| |operand| + 300 u sum |dy| |operand|, and half a step where the result is bf16 (dx)"""
+    from yolov5m_amd.model import CBL, _ConvKeptFn
+    cin, cout, k, s = case
+    torch.manual_seed(129)
+    m = CBL(cin, cout, k, s, k // 2, norm_groups=8, keep=keep).to(DEV)
+    m.compute_dtype = "bf16"
+    with torch.no_grad():
+        m.cbl[1].weight.copy_(_params(cout, 130)[0])
+        m.cbl[1].bias.copy_(_params(cout, 130)[1])
+    x = torch.randn(2, cin, 10, 6, generator=torch.Generator().manual_seed(131)).to(DEV).requires_grad_()
+    z = m(x)
+    w = torch.randn(z.shape, generator=torch.Generator().manual_seed(132)).to(DEV)
+    (z * w).sum().backward()
+    half, conv = 2.0 ** -8, dict(stride=s, padding=k // 2)
+    b64 = lambda t: t.detach().cpu().bfloat16().double()
+    xd, wd = b64(x), b64(m.cbl[0].weight)
+    y = _ConvKeptFn.apply(x.detach(), m.cbl[0].weight.detach(), m)
+    ref = F.conv2d(xd, wd, **conv)
+    assert y.dtype == torch.bfloat16
+    assert ((y.cpu().double() - ref).abs() <= half * ref.abs() + (1 + half) * 300 * U * F.conv2d(xd.abs(), wd.abs(), **conv)).all()
+    nhwc = lambda t: t.contiguous(memory_format=torch.channels_last)
+    norm = Exact(y, 8, m.cbl[1].weight, m.cbl[1].bias, 1e-3, "silu", None if keep == "x" else stored_values(y, keep)[0], w.bfloat16())
+    near(norm, z.detach().bfloat16(), "z")
+    assert torch.equal(z.detach().bfloat16().float(), z.detach())
+    near(norm, m.cbl[1].weight.grad, "dgamma")
+    near(norm, m.cbl[1].bias.grad, "dbeta")
+    img = lambda t: t.reshape(2, *y.shape[2:], cout).movedim(-1, 1)
+    dy, err = img(norm.dx), img(norm.dx_tol + half * (norm.dx.abs() + norm.dx_tol))
+    xk = xd if keep == "x" else stored_values(nhwc(x.detach().bfloat16()), keep)[0].movedim(-1, 1)
+    for got, op, grad, rnd in ((x.grad, wd, lambda o, d: torch.nn.grad.conv2d_input(xd.shape, o, d, **conv), half),
+                               (m.cbl[0].weight.grad, xk, lambda o, d: torch.nn.grad.conv2d_weight(o, wd.shape, d, **conv), 0.0)):
+        want = grad(op, dy)
+        tol = grad(op.abs(), err + 300 * U * dy.abs())
+        assert ((got.cpu().double() - want).abs() <= tol + rnd * (want.abs() + tol)).all()
