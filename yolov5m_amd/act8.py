@@ -5,8 +5,8 @@
     dw, db = act8_wgrad(dy, kept)           # pointwise convolution: dw (Cout, C), from the 8-bit form directly
 
 Every 32 consecutive channels of a row share one scale 2^e (one byte), e the smallest exponent >= -117 that holds the block's largest
-magnitude; the codes are e4m3 (3 mantissa bits: relative error <= 2^-4 down to 2^-15 of the block's maximum) or int8 (absolute error
-<= 2^-7 of the block's maximum), rounded to nearest even. 1 + 1/32 bytes per element. Magnitudes above 1.875 * 2^E (E the largest
+magnitude; the codes are e4m3 (3 mantissa bits: relative error <= 2^-4 down to 2^-13 of the block's maximum) or int8 (absolute error
+<= 1/127 of the block's maximum), rounded to nearest even; both where e is above -117. 1 + 1/32 bytes per element. Magnitudes above 1.875 * 2^E (E the largest
 exponent of x's type) are held as that value; a block with a NaN or an infinity reads back as NaN throughout.
 
 The rows of a tensor are its positions (n, *spatial), each C consecutive values: torch.channels_last tensors, (N, L, C) token tensors
@@ -157,7 +157,7 @@ def act8_load(kept):
 def act8_wgrad(dy, kept, bias=False):
     """weight gradient of a pointwise convolution (or linear layer) whose input was kept in 8 bits: dy (N, Cout, *spatial) over the
     same positions, channels last -> dw (Cout, C) f32, db (Cout,) f32 or None. Sums run over the values that were kept, products are
-    exact, accumulation is f32 (joined in f64); dy may be of another type than what was stored."""
+    exact, accumulation is f32 (joined in f64); dy may be of another type than what was stored, and infinite: dw is what the sums are then."""
     same_device(kept.q, dy=dy)
     n, s, cout, dn, dr = rows_of(dy, "dy")
     if dy.shape[0] != kept.shape[0] or dy.shape[2:] != kept.shape[2:]:

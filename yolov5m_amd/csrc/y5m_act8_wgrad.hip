@@ -2,7 +2,7 @@
 //
 // GEMM with K = rows (up to millions) and both operands row-major along K, as they lie in memory. Arithmetic: an 8-bit value times its
 // power-of-two scale has at most 8 significant bits, so it IS a bf16 value; dY in bf16 is one, in fp16 (11 bits) the exact sum of two
-// and in f32 (24 bits) of three bf16 values. Products of bf16 MFMAs are exact in f32, so every type runs on the bf16 matrix cores
+// and in f32 (24 bits) of three bf16 values (infinities and what rounds to one are taken again, in limited pieces). Products of bf16 MFMAs are exact in f32, so every type runs on the bf16 matrix cores
 // with f32 accumulation, and nothing is rounded before the sum (f32 MFMA: 1/16 of the rate).
 //
 // An MFMA operand wants 8 consecutive k (rows) of ONE channel per lane, memory has 8 channels of one row next to each other. No LDS

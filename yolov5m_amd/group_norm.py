@@ -7,8 +7,8 @@ with few images per GPU, next to the network's BatchNorm + SiLU (ops.bn_act, ops
 
 `keep` says what the forward leaves for the backward: None (inference: nothing), "x" (the input itself, not copied), or "e4m3" / "int8"
 (the input in 8 bits, written in the same pass; act8.py has the form). From the 8-bit form the backward takes the gradient at the values
-that were kept, with the forward's mean and rstd; x itself can be freed or overwritten. Statistics are f32 and joined in f64, in a
-fixed order. Types: float32, bfloat16, float16 for x / z / dz / dx; weight and bias are read as float32, their gradients are float32.
+that were kept, with the forward's mean and rstd; x itself can be freed or overwritten. Statistics are right to f32's rounding for
+finite inputs up to half of the type's largest, whatever their spread, and joined in f64 in a fixed order. Types: float32, bfloat16, float16 for x / z / dz / dx; weight and bias are read as float32, their gradients are float32.
 """
 import torch
 import torch.nn as nn

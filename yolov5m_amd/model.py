@@ -28,7 +28,9 @@ class CBL(nn.Module):
 
     norm_groups: GroupNorm over that many groups in BatchNorm's place (statistics of one image: small batches), for blocks built from
     these modules; the whole-model engine runs the BatchNorm network. keep (with norm_groups): what a training forward leaves for its
-    backward -- "x" (the convolution's input and output whole) or "e4m3" / "int8" (both in 8 bits, act8.py)."""
+    backward -- "x" (the convolution's input and output whole) or "e4m3" / "int8" (both in 8 bits, act8.py); nothing is kept where no
+    gradient is wanted. As with BatchNorm, a module's own forward goes through ops.py, which takes and returns NCHW f32, converts the layout
+    on both sides of every convolution and waits for the device: for parity and memory, not for speed, and not for graph capture."""
 
     def __init__(self, in_channels, out_channels, kernel_size, stride, padding, norm_groups=None, keep="x"):
         super().__init__()
