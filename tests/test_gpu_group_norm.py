@@ -829,3 +829,21 @@ def test_cbl_with_group_norm_in_bf16(case, keep):
         want = grad(op, dy)
         tol = grad(op.abs(), err + 300 * U * dy.abs())
         assert ((got.cpu().double() - want).abs() <= tol + rnd * (want.abs() + tol)).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [4, 50, 5000])
+def test_half_of_the_largest_value(rows, dtype):
+    """maps of +-1.6e38: rstd is below f32's normal range (its step there, 2^-149 of 6e-39, is 4 u) and z is +-1"""
+    from yolov5m_amd.group_norm import group_norm_act, group_norm_act_backward
+    x = torch.full((2, rows, 16), 1.6e38)
+    x[:, ::2, ::3] = -1.6e38
+    x[:, 1::2, 1::3] = -1.6e38
+    x = x.to(DT[dtype]).movedim(-1, 1).to(DEV)
+    dz = (_rows((2, 16, rows), "f32", 133) * 1e20).to(DT[dtype])
+    ref = Exact(x, 4, None, None, 1e-5, None, None, dz)
+    z, saved = group_norm_act(x, 4, act=None, keep="x")
+    near(ref, z, "z")
+    assert ((saved.rstd.cpu().double().flatten() - ref.rstd).abs() <= 8 * U * ref.rstd).all()
+    for got, what in zip(group_norm_act_backward(dz, saved), ("dx", "dgamma", "dbeta")):
+        near(ref, got, what)
