@@ -847,3 +847,15 @@ def test_half_of_the_largest_value(rows, dtype):
     assert ((saved.rstd.cpu().double().flatten() - ref.rstd).abs() <= 8 * U * ref.rstd).all()
     for got, what in zip(group_norm_act_backward(dz, saved), ("dx", "dgamma", "dbeta")):
         near(ref, got, what)
+
+
+@pytest.mark.parametrize("rows", [1, 40, 5000])
+def test_equal_values_far_from_zero(rows):
+    """groups of one value in 16 bits: xhat is 0 and z = act(bias) to the type's rounding, however large the value and rstd are"""
+    from yolov5m_amd.group_norm import group_norm_act
+    ga, be = _params(16, 134)
+    for dtype, value, eps in (("bf16", 1e10, 1e-5), ("bf16", -1e37, 1e-5), ("bf16", 1.5e38, 1e-3), ("fp16", 6e4, 1e-12), ("bf16", 300.0, 1e-14)):
+        x = torch.full((2, rows, 16), value).to(DT[dtype]).movedim(-1, 1).to(DEV)
+        z, _ = group_norm_act(x, 4, ga, be, eps=eps, act=None)
+        b = be.to(DT[dtype]).view(1, 16, 1).expand(2, 16, rows)
+        assert torch.equal(z, b), (dtype, value, float((z - b).abs().max()))

@@ -373,8 +373,16 @@ template <int DT> struct GnAffine {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             a[i] = k.rstd[i] * k.gamma[i];
-            if constexpr (DT == Y5M_F32) { m[i] = k.mean[i]; b[i] = k.beta[i]; }
-            else b[i] = fmaf(-k.mean[i], a[i], k.beta[i]);
+            if constexpr (DT == Y5M_F32) {
+                m[i] = k.mean[i];
+                b[i] = k.beta[i];
+            } else {
+                // above 2^27 the group's values are all the same: 16-bit ones that differ spread over 2^-11 / sqrt(K) of the mean at least,
+                // K < 2^31. xhat is 0 then, and mean a would only leave its rounding, or infinity
+                const bool same = fabsf(k.mean[i]) * k.rstd[i] > 0x1p27f;
+                if (same) a[i] = 0.f;
+                b[i] = same ? k.beta[i] : fmaf(-k.mean[i], a[i], k.beta[i]);
+            }
         }
     }
     __device__ __forceinline__ float operator()(float v, int i) const {
@@ -673,7 +681,8 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_reduce_kernel(const GnParam
         if (DT == Y5M_BF16 && !(fabsf(s1) < INFINITY)) far = 1;
     });
     if constexpr (DT == Y5M_BF16) {
-        // (asked last, where nothing of the loop is held any more: asked before it, or between it and the join, it cost 4 to 10 %)
+        // (asked last, where nothing of the loop is held any more: a step over 64 x 160 x 160 x 96 in int8 takes 448 us, 493 with the statistics
+        // asked in front of the rows, 455 to 460 between the loop and the join)
         __syncthreads();
         if (__builtin_expect(far, 0)) {
             for (int i = 0; i < 8; ++i) {
